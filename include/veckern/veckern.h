@@ -248,6 +248,74 @@ int vk_pq_encode_device(const float* d_centroids, size_t d, size_t m, const floa
  * nearest of the 256 centroids (256 x dsub) to sub-vector i (sub: n x dsub). Host buffers. */
 int vk_pq_assign(const float* centroids, size_t dsub, const float* sub, size_t n, uint32_t* assign);
 
+/* Attention to the states of found rows. A model that answers with what a search found attends to an encoder's states of
+ * it: the states are rows of passages, keys and values [bank][length][kv_heads][head_dim], of which row n holds
+ * lengths[n] positions (all `length` where lengths is NULL; values are taken into [0, length]). Request b attends to the
+ * rows rows[b * rows_stride[0] + r * rows_stride[1]], r < passages: the strides let a search's vk_neighbor records be read
+ * where they are (rows = &out[0].id, strides {2 k, 2}); an id outside [0, bank) holds nothing, as the padding id -1 does.
+ * Where rows is NULL, bank == batch * passages and request b has the rows b * passages + r.
+ *   L[t, key] = scale * q[t] . k[key] + table[bucket(position of key in its row - (t + q_start + q_starts[b]))][head]
+ *   P = softmax of L over the keys there are,  out = P v,  lse = log of the sum of exp(L), in two parts: its value in 32
+ *   bits and what that rounding left off (which matters where a whole row's bias is of a size that swallows the rest)
+ * A token with no key, or with no L above -inf, gets out = 0 and lse = -inf, and gradients of 0. Query head h reads key head
+ * h / (heads / kv_heads). All of a tensor's elements have the type `type`; products are accumulated and statistics held in
+ * 32 bits, P and its gradient are rounded to `type` where they are multiplied again.
+ * No counterpart in the reference. Unlike the searchers' calls these are asynchronous: they launch on the caller's stream
+ * (a hipStream_t; NULL: the default stream of the current device), allocate nothing and can be captured in a graph. The
+ * workspace (16-byte aligned device memory of at least the bytes that the matching call states for the same arguments;
+ * NULL where that is 0) must stay until the launched work is done and be used by one such call at a time. Results are
+ * deterministic. Errors: VK_ERR_INVALID_ARGUMENT, before any launch. */
+enum vk_type { VK_F16 = 0, VK_BF16 = 1 };
+
+/* A tensor [batch or bank][tokens or length][heads][head_dim]: element strides of the first three dimensions, none negative,
+ * multiples of 8; the last is contiguous; data 16-byte aligned. A stride of a dimension of size 1 is not looked at. A stride
+ * of 0 repeats an input; outputs must not overlap. */
+typedef struct vk_tensor {
+    void* data;
+    int64_t stride[3];
+} vk_tensor;
+
+typedef struct vk_attention {
+    int type;                            /* vk_type */
+    size_t batch, tokens, heads;         /* of the queries */
+    size_t kv_heads;                     /* divides heads */
+    size_t head_dim;                     /* a multiple of 8, at most 128 */
+    size_t passages, length, bank;       /* rows a request attends to, positions of a row, rows there are (< 2^31) */
+    float scale;                         /* finite, not negative */
+    vk_tensor q, k, v, out;              /* out: written by vk_attend, read by vk_attend_backward */
+    const int32_t* rows;                 /* device, or NULL */
+    int64_t rows_stride[2];
+    const int32_t* lengths;              /* device, [bank], or NULL */
+    float* lse;                          /* device, [batch][heads][tokens][2]; may be NULL for vk_attend */
+    /* The position bias: table [buckets][heads] (device, `type`, any strides), NULL for none. Of a side's buckets (all, or
+     * half of them for each direction where two_sided) the first half hold one distance each and the others grow by a
+     * common factor up to max_distance (vk_bias_bucket). buckets <= 256, max_distance <= 1024. */
+    const void* table;
+    int64_t table_stride[2];
+    size_t buckets, max_distance;
+    int two_sided;
+    int64_t q_start;                     /* position of token 0, |q_start| < 2^30 */
+    const int32_t* q_starts;             /* device, [batch], added to q_start; or NULL */
+} vk_attention;
+
+typedef struct vk_attention_grad {
+    vk_tensor d_out, d_q, d_k, d_v;      /* d_k, d_v: NULL data where rows is given (the bank then is a constant) */
+    void* d_table;                       /* [buckets][heads], contiguous, `type`; NULL without a table */
+} vk_attention_grad;
+
+/* The bucket of distance = key position - query position: with n = buckets, or n = buckets / 2 (buckets even) where
+ * two_sided, a = |distance| (one-sided: max(-distance, 0)) and e = n / 2, it is a for a < e and else
+ * min(n - 1, e + floor(log(a / e) / log(max_distance / e) * (n - e))), taken exactly; plus n where two_sided and
+ * distance > 0. Host only. */
+int vk_bias_bucket(int64_t distance, size_t buckets, size_t max_distance, int two_sided, int* bucket);
+int vk_attend_workspace(const vk_attention* a, size_t* bytes);
+int vk_attend(const vk_attention* a, void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients of a loss whose gradient by `out` is d_out, given the forward's out and lse. All of d_q, d_k, d_v and
+ * d_table are written (zeros where nothing was attended to); d_k and d_v sum over the query heads that share a key head. */
+int vk_attend_backward_workspace(const vk_attention* a, size_t* bytes);
+int vk_attend_backward(const vk_attention* a, const vk_attention_grad* g, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

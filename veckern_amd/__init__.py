@@ -85,6 +85,26 @@ class _ScanKernel(ctypes.Structure):
                 ("votes", ctypes.c_int)]
 
 
+class _Tensor(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64 * 3)]
+
+
+class _Attention(ctypes.Structure):
+    _fields_ = [("type", ctypes.c_int), ("batch", ctypes.c_size_t), ("tokens", ctypes.c_size_t),
+                ("heads", ctypes.c_size_t), ("kv_heads", ctypes.c_size_t), ("head_dim", ctypes.c_size_t),
+                ("passages", ctypes.c_size_t), ("length", ctypes.c_size_t), ("bank", ctypes.c_size_t),
+                ("scale", ctypes.c_float), ("q", _Tensor), ("k", _Tensor), ("v", _Tensor), ("out", _Tensor),
+                ("rows", ctypes.c_void_p), ("rows_stride", ctypes.c_int64 * 2), ("lengths", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64 * 2),
+                ("buckets", ctypes.c_size_t), ("max_distance", ctypes.c_size_t), ("two_sided", ctypes.c_int),
+                ("q_start", ctypes.c_int64), ("q_starts", ctypes.c_void_p)]
+
+
+class _AttentionGrad(ctypes.Structure):
+    _fields_ = [("d_out", _Tensor), ("d_q", _Tensor), ("d_k", _Tensor), ("d_v", _Tensor),
+                ("d_table", ctypes.c_void_p)]
+
+
 class _DeviceInfo(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 256), ("arch", ctypes.c_char * 64), ("sm_count", ctypes.c_int),
                 ("peak_bandwidth_gbs", ctypes.c_double), ("max_smem_per_block", ctypes.c_size_t),
@@ -141,6 +161,13 @@ _SIGNATURES = {
                                  ctypes.POINTER(_Timings)]),
     "vk_rerank_device": (ctypes.c_int, [_P, _P, ctypes.c_size_t, _P, ctypes.c_size_t, ctypes.c_size_t, _P,
                                         ctypes.POINTER(_Timings)]),
+    "vk_bias_bucket": (ctypes.c_int, [ctypes.c_int64, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_int,
+                                      ctypes.POINTER(ctypes.c_int)]),
+    "vk_attend_workspace": (ctypes.c_int, [ctypes.POINTER(_Attention), ctypes.POINTER(ctypes.c_size_t)]),
+    "vk_attend": (ctypes.c_int, [ctypes.POINTER(_Attention), _P, ctypes.c_size_t, _P]),
+    "vk_attend_backward_workspace": (ctypes.c_int, [ctypes.POINTER(_Attention), ctypes.POINTER(ctypes.c_size_t)]),
+    "vk_attend_backward": (ctypes.c_int, [ctypes.POINTER(_Attention), ctypes.POINTER(_AttentionGrad), _P,
+                                          ctypes.c_size_t, _P]),
 }
 
 _lib = None

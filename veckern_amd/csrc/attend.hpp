@@ -1,0 +1,69 @@
+// Attention over rows of encoder states: arguments and launches shared by the C ABI (attend_capi.hip) and the kernels
+// (attend_forward*.hip, attend_backward*.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace vk {
+
+constexpr int kMostEdges = 128;      // bucket edges of a one-sided bias of 256 buckets
+constexpr int kMostDistance = 1024;  // largest max_distance: the bias by distance, and its gradient, are held in LDS
+constexpr int kKeyTile = 64;         // keys that a block of the tile kernels holds at once
+constexpr int kColumns = 128;        // query columns of a block of the tile kernels
+
+// A tensor [outer][middle][head][d]: element strides, d contiguous.
+struct AttendView {
+    void* p = nullptr;
+    int64_t outer = 0, middle = 0, head = 0;
+};
+
+// Position bias by buckets. The distance x = key position - query position falls into the bucket
+//   (two-sided and x > 0 ? side : 0) + (a < side / 2 ? a : side / 2 + (number of edges <= a)),   a = |x| or max(-x, 0).
+struct AttendBias {
+    const void* table = nullptr;  // [buckets][heads], of the queries' type; nullptr: no bias
+    int64_t bucket_stride = 0, head_stride = 0;
+    int buckets = 0, side = 0, edges = 0;
+    int far = 0;  // from this distance on, and beyond, the last bucket of a side
+    bool two_sided = false;
+    int edge[kMostEdges];
+};
+
+struct AttendArgs {
+    AttendView q, k, v, out;      // q, out: [batch][tokens][heads][d]; k, v: [bank][length][kv_heads][d]
+    float2* lse = nullptr;        // [batch][heads][tokens] (value, what its rounding left off); may be nullptr in the forward pass
+    const int32_t* rows = nullptr;  // [batch][passages] by rows_outer, rows_step; nullptr: b * passages + r
+    int64_t rows_outer = 0, rows_step = 0;
+    const int32_t* lengths = nullptr;   // [bank]; nullptr: all `length`
+    const int32_t* q_start = nullptr;   // [batch], added to q_start_all
+    int q_start_all = 0;
+    int batch = 0, tokens = 0, heads = 0, kv_heads = 0, d = 0, passages = 0, length = 0;
+    int64_t bank = 0;
+    float scale = 0.f;            // positive, so that -inf * scale is -inf (0 is taken as 1e-37)
+    AttendBias bias;
+    // How the work is laid out. pack: query heads of one key head that share a block's columns (column = token * pack + head).
+    int pack = 1, splits = 1, tiles_per_split = 0;
+    float* part = nullptr;   // splits > 1: [splits][batch][heads / pack][tokens * pack][d] unnormalised sums ...
+    float2* stat = nullptr;  // ... and [splits][...][tokens * pack] (maximum, sum)
+};
+
+struct AttendGradArgs {
+    AttendArgs a;                 // out: the forward's result, lse: its statistics
+    AttendView d_out, d_q, d_k, d_v;
+    float scale = 0.f;            // the logits' own, which may be 0
+    float* delta = nullptr;       // workspace [batch][heads][tokens]
+    float* table_part = nullptr;  // workspace [batch * column tiles][heads][buckets]
+    void* d_table = nullptr;      // [buckets][heads], contiguous
+};
+
+enum AttendType { kAttendF16 = 0, kAttendBf16 = 1 };
+
+hipError_t launch_attend_forward(const AttendArgs& a, int type, hipStream_t stream);
+hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stream);
+// Writes d_q (and delta, and the table's partial sums).
+hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream);
+hipError_t launch_attend_grad_kv(const AttendGradArgs& g, int type, hipStream_t stream);
+hipError_t launch_attend_grad_table(const AttendGradArgs& g, int type, int parts, hipStream_t stream);
+
+}  // namespace vk

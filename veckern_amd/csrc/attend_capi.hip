@@ -1,0 +1,259 @@
+// C ABI of the attention over found rows (vk_attend, vk_attend_backward): checks, the plan of a call, and its launches.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "attend.hpp"
+#include "errors.hpp"
+
+namespace vk {
+
+#define VK_ATTEND_INSTANCES(type, size)                                              \
+    hipError_t attend_forward_##type##_##size(const AttendArgs& a, hipStream_t stream);     \
+    hipError_t attend_grad_q_##type##_##size(const AttendGradArgs& g, hipStream_t stream);  \
+    hipError_t attend_grad_kv_##type##_##size(const AttendGradArgs& g, hipStream_t stream);
+VK_ATTEND_INSTANCES(bf16, 64)
+VK_ATTEND_INSTANCES(bf16, 128)
+VK_ATTEND_INSTANCES(f16, 64)
+VK_ATTEND_INSTANCES(f16, 128)
+
+hipError_t launch_attend_forward(const AttendArgs& a, int type, hipStream_t stream) {
+    if (type == kAttendBf16) return a.d <= 64 ? attend_forward_bf16_64(a, stream) : attend_forward_bf16_128(a, stream);
+    return a.d <= 64 ? attend_forward_f16_64(a, stream) : attend_forward_f16_128(a, stream);
+}
+hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream) {
+    if (type == kAttendBf16) return g.a.d <= 64 ? attend_grad_q_bf16_64(g, stream) : attend_grad_q_bf16_128(g, stream);
+    return g.a.d <= 64 ? attend_grad_q_f16_64(g, stream) : attend_grad_q_f16_128(g, stream);
+}
+hipError_t launch_attend_grad_kv(const AttendGradArgs& g, int type, hipStream_t stream) {
+    if (type == kAttendBf16) return g.a.d <= 64 ? attend_grad_kv_bf16_64(g, stream) : attend_grad_kv_bf16_128(g, stream);
+    return g.a.d <= 64 ? attend_grad_kv_f16_64(g, stream) : attend_grad_kv_f16_128(g, stream);
+}
+
+}  // namespace vk
+
+namespace {
+
+using vk::AttendArgs;
+using vk::AttendBias;
+using vk::AttendGradArgs;
+using vk::AttendView;
+using vk::fail;
+using vk::guarded;
+
+void valid(bool condition, const char* message) {
+    if (!condition) fail(VK_ERR_INVALID_ARGUMENT, message);
+}
+
+constexpr size_t kMost = (size_t(1) << 31) - 1;
+
+// The bucket layout of vk_bias_bucket. The edge of bucket e + i is the least x with x >= e (max_distance / e)^(i / (n - e)):
+// where that power is a whole number, the logarithms' rounding must not move the edge past it.
+AttendBias bias_of(size_t buckets, size_t max_distance, bool two_sided) {
+    valid(buckets <= 2 * vk::kMostEdges, "the bias has more than 256 buckets");
+    valid(!two_sided || buckets % 2 == 0, "a two-sided bias needs an even number of buckets");
+    AttendBias s;
+    s.two_sided = two_sided;
+    s.buckets = static_cast<int>(buckets);
+    s.side = s.buckets / (two_sided ? 2 : 1);
+    valid(s.side >= 2, "the bias needs at least two buckets a side");
+    const int e = s.side / 2, w = s.side - e;
+    valid(max_distance > static_cast<size_t>(e), "max_distance must exceed the buckets of one distance each");
+    valid(max_distance <= vk::kMostDistance, "max_distance is more than 1024");
+    s.edges = w - 1;
+    for (int i = 1; i < w; ++i) {
+        const long double x = e * std::pow(static_cast<long double>(max_distance) / e, static_cast<long double>(i) / w);
+        const long double whole = std::round(x);
+        s.edge[i - 1] = static_cast<int>(std::fabs(x - whole) < 1e-12L * x ? whole : std::ceil(x));
+    }
+    s.far = s.edges ? s.edge[s.edges - 1] : e;
+    return s;
+}
+
+struct Dim {
+    size_t outer, middle, head;
+};
+
+AttendView view_of(const vk_tensor& t, const Dim& size, const char* name) {
+    const std::string n = name;
+    const bool none = size.outer == 0 || size.middle == 0 || size.head == 0;
+    AttendView v;
+    v.p = t.data;
+    const size_t sizes[3] = {size.outer, size.middle, size.head};
+    int64_t stride[3];
+    for (int i = 0; i < 3; ++i) {
+        stride[i] = sizes[i] > 1 ? t.stride[i] : 0;
+        if (stride[i] < 0 || stride[i] % 8) fail(VK_ERR_INVALID_ARGUMENT, n + ": strides must be multiples of 8 elements and not negative");
+    }
+    // a tile's rows are reached by 32-bit offsets
+    if (stride[1] >= (int64_t(1) << 23)) fail(VK_ERR_INVALID_ARGUMENT, n + ": the stride between positions is 2^23 elements or more");
+    if (!none && !t.data) fail(VK_ERR_INVALID_ARGUMENT, n + " is NULL");
+    if (reinterpret_cast<uintptr_t>(t.data) % 16) fail(VK_ERR_INVALID_ARGUMENT, n + " is not 16-byte aligned");
+    v.outer = stride[0];
+    v.middle = stride[1];
+    v.head = stride[2];
+    return v;
+}
+
+// Checks a call's arguments; `out` only where the call has it.
+AttendArgs args_of(const vk_attention* x, bool tensors) {
+    valid(x != nullptr, "arguments are NULL");
+    valid(x->type == VK_F16 || x->type == VK_BF16, "type must be VK_F16 or VK_BF16");
+    valid(x->head_dim >= 8 && x->head_dim <= 128 && x->head_dim % 8 == 0, "head_dim must be a multiple of 8 and at most 128");
+    valid(x->heads > 0 && x->kv_heads > 0 && x->heads % x->kv_heads == 0, "heads must be a multiple of kv_heads");
+    valid(x->batch <= kMost && x->tokens <= kMost && x->passages <= kMost && x->length <= kMost && x->bank <= kMost && x->heads <= 65536,
+          "a size is too large");
+    valid(x->tokens * x->heads <= kMost / 2 && (x->length + vk::kKeyTile) / vk::kKeyTile * x->passages <= kMost / 2 &&
+              x->length <= kMost / 2, "a size is too large");
+    valid(std::isfinite(x->scale) && x->scale >= 0.f, "scale must be finite and not negative");
+    valid(x->rows || x->bank == x->batch * x->passages, "without rows, bank must be batch * passages");
+    valid(x->q_start > -(int64_t(1) << 30) && x->q_start < (int64_t(1) << 30), "q_start is out of range");
+    AttendArgs a;
+    a.batch = static_cast<int>(x->batch);
+    a.tokens = static_cast<int>(x->tokens);
+    a.heads = static_cast<int>(x->heads);
+    a.kv_heads = static_cast<int>(x->kv_heads);
+    a.d = static_cast<int>(x->head_dim);
+    a.passages = static_cast<int>(x->passages);
+    a.length = static_cast<int>(x->length);
+    a.bank = static_cast<int64_t>(x->bank);
+    a.scale = std::max(x->scale, 1e-37f);
+    a.rows = x->rows;
+    a.rows_outer = x->rows_stride[0];
+    a.rows_step = x->rows_stride[1];
+    a.lengths = x->lengths;
+    a.q_start = x->q_starts;
+    a.q_start_all = static_cast<int>(x->q_start);
+    a.lse = reinterpret_cast<float2*>(x->lse);
+    valid(reinterpret_cast<uintptr_t>(x->lse) % 8 == 0, "lse is not 8-byte aligned");
+    if (x->table) {
+        a.bias = bias_of(x->buckets, x->max_distance, x->two_sided != 0);
+        a.bias.table = x->table;
+        a.bias.bucket_stride = x->table_stride[0];
+        a.bias.head_stride = x->table_stride[1];
+        valid(a.bias.bucket_stride >= 0 && a.bias.head_stride >= 0, "the bias table's strides must not be negative");
+    }
+    if (tensors) {
+        const Dim q{x->batch, x->tokens, x->heads}, k{x->bank, x->length, x->kv_heads};
+        a.q = view_of(x->q, q, "q");
+        a.out = view_of(x->out, q, "out");
+        a.k = view_of(x->k, k, "k");
+        a.v = view_of(x->v, k, "v");
+    }
+    return a;
+}
+
+// Blocks that fill the card's 256 CUs twice: below that the keys are split.
+constexpr int64_t kEnoughBlocks = 512;
+
+void plan_forward(AttendArgs& a) {
+    const int share = a.heads / a.kv_heads;
+    a.pack = share;
+    if (a.bias.table && static_cast<size_t>(share) * (2 * a.bias.far + 7) * sizeof(float) > 16384) a.pack = 1;
+    const int tiles = (a.length + vk::kKeyTile - 1) / vk::kKeyTile * a.passages;
+    const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + vk::kColumns - 1) / vk::kColumns * (a.heads / a.pack) * a.batch;
+    a.splits = 1;
+    a.tiles_per_split = tiles;
+    if (blocks > 0 && blocks < kEnoughBlocks && tiles > 1) {
+        const int64_t wanted = std::min<int64_t>((kEnoughBlocks + blocks - 1) / blocks, tiles);
+        a.tiles_per_split = static_cast<int>((tiles + wanted - 1) / wanted);
+        a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+    }
+}
+size_t query_rows(const AttendArgs& a) { return static_cast<size_t>(a.batch) * a.heads * a.tokens; }
+size_t align(size_t x) { return (x + 15) / 16 * 16; }
+size_t forward_bytes(const AttendArgs& a) {
+    return a.splits == 1 ? 0 : align(a.splits * query_rows(a) * a.d * sizeof(float)) + a.splits * query_rows(a) * sizeof(float2);
+}
+int table_parts(const AttendArgs& a) { return (a.tokens + vk::kColumns - 1) / vk::kColumns * a.batch; }
+size_t table_bytes(const AttendArgs& a) {
+    return a.bias.table ? static_cast<size_t>(table_parts(a)) * a.heads * a.bias.buckets * sizeof(float) : 0;
+}
+size_t backward_bytes(const AttendArgs& a) { return align(query_rows(a) * sizeof(float)) + table_bytes(a); }
+
+void check_workspace(void* workspace, size_t bytes, size_t needed) {
+    valid(bytes >= needed && (workspace || !needed), "the workspace is too small");
+    valid(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace is not 16-byte aligned");
+}
+
+}  // namespace
+
+VK_EXPORT int vk_bias_bucket(int64_t distance, size_t buckets, size_t max_distance, int two_sided, int* bucket) {
+    return guarded([&] {
+        valid(bucket != nullptr, "bucket is NULL");
+        const AttendBias s = bias_of(buckets, max_distance, two_sided != 0);
+        const int64_t far = s.far;
+        const int x = static_cast<int>(std::min(std::max(distance, -far), far));
+        const int a = two_sided ? std::abs(x) : std::max(-x, 0), e = s.side / 2;
+        int b = a;
+        if (a >= e) {
+            b = e;
+            for (int i = 0; i < s.edges; ++i) b += s.edge[i] <= a;
+        }
+        *bucket = b + (two_sided && distance > 0 ? s.side : 0);
+    });
+}
+
+VK_EXPORT int vk_attend_workspace(const vk_attention* x, size_t* bytes) {
+    return guarded([&] {
+        valid(bytes != nullptr, "bytes is NULL");
+        AttendArgs a = args_of(x, false);
+        plan_forward(a);
+        *bytes = forward_bytes(a);
+    });
+}
+
+VK_EXPORT int vk_attend(const vk_attention* x, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        AttendArgs a = args_of(x, true);
+        plan_forward(a);
+        check_workspace(workspace, workspace_bytes, forward_bytes(a));
+        if (!query_rows(a)) return;
+        if (a.splits > 1) {
+            a.part = static_cast<float*>(workspace);
+            a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) + align(a.splits * query_rows(a) * a.d * sizeof(float)));
+        }
+        const auto on = static_cast<hipStream_t>(stream);
+        VK_HIP(vk::launch_attend_forward(a, x->type, on));
+        if (a.splits > 1) VK_HIP(vk::launch_attend_combine(a, x->type, on));
+    });
+}
+
+VK_EXPORT int vk_attend_backward_workspace(const vk_attention* x, size_t* bytes) {
+    return guarded([&] {
+        valid(bytes != nullptr, "bytes is NULL");
+        *bytes = backward_bytes(args_of(x, false));
+    });
+}
+
+VK_EXPORT int vk_attend_backward(const vk_attention* x, const vk_attention_grad* y, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+    return guarded([&] {
+        valid(y != nullptr, "gradients are NULL");
+        AttendGradArgs g;
+        g.a = args_of(x, true);
+        AttendArgs& a = g.a;
+        const Dim q{x->batch, x->tokens, x->heads}, k{x->bank, x->length, x->kv_heads};
+        g.d_out = view_of(y->d_out, q, "d_out");
+        g.d_q = view_of(y->d_q, q, "d_q");
+        if (x->rows) {
+            valid(!y->d_k.data && !y->d_v.data, "rows of a bank are constants: d_k and d_v must be NULL where rows is given");
+        } else {
+            g.d_k = view_of(y->d_k, k, "d_k");
+            g.d_v = view_of(y->d_v, k, "d_v");
+        }
+        valid(!query_rows(a) || a.lse, "lse is NULL");
+        valid(!a.bias.table || y->d_table, "d_table is NULL");
+        valid(a.bias.table || !y->d_table, "d_table is given without a table");
+        g.d_table = y->d_table;
+        g.scale = x->scale;
+        check_workspace(workspace, workspace_bytes, backward_bytes(a));
+        g.delta = static_cast<float*>(workspace);
+        g.table_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align(query_rows(a) * sizeof(float)));
+        a.pack = a.bias.table ? 1 : a.heads / a.kv_heads;
+        const auto on = static_cast<hipStream_t>(stream);
+        if (query_rows(a)) VK_HIP(vk::launch_attend_grad_q(g, x->type, on));
+        if (!x->rows && x->bank && x->length) VK_HIP(vk::launch_attend_grad_kv(g, x->type, on));
+        if (a.bias.table) VK_HIP(vk::launch_attend_grad_table(g, x->type, table_parts(a), on));
+    });
+}

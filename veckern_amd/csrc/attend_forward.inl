@@ -1,0 +1,199 @@
+// The forward pass by tiles: O = softmax(scale Q K^T + bias) V, one pass over the keys with the running maximum and sum.
+//
+// A block of four waves holds 128 query columns, each wave 32 of them, and walks the key tiles of its request; a key tile (64
+// rows of K and of V) is staged in LDS for all four, the next one's loads in flight meanwhile. The products are taken
+// transposed, S^T = K Q^T and O^T = V^T P^T: a lane then holds one query column of the logits, its maximum and sum need one
+// exchange with the lane 32 further, and the rounded weights are the second product's operand where they are.
+//
+// P is rounded to the inputs' type for the second product (the matrix instructions take 16-bit operands); the sum that
+// normalises it, the maximum and the output are held in 32 bits. The weights are relative to a maximum that is only raised
+// when it grew by more than kSlack: the output's rescaling is rare, and P <= e^kSlack keeps its relative precision in either
+// type.
+#include "attend_tile.hpp"
+
+namespace vk::attend {
+
+constexpr float kSlack = 5.f;
+
+template <class E, int DP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
+    constexpr int kSteps = DP / 16, kParts = DP / 32;
+    __shared__ s16x8 tile[2][2][kKeyTile * DP / 8];
+    extern __shared__ float bias_held[];
+
+    const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
+    const int columns = a.tokens * a.pack, column_tiles = (columns + kColumns - 1) / kColumns, groups = a.heads / a.pack;
+    int place = xcd_place(blockIdx.x, gridDim.x);
+    const int column_tile = place % column_tiles;
+    place /= column_tiles;
+    const int split = place % a.splits;
+    place /= a.splits;
+    const int group = place % groups, b = place / groups;
+    const int kv_head = group * a.pack / (a.heads / a.kv_heads);
+
+    const int c = column_tile * kColumns + wave * 32 + lane % 32;
+    const int token = c / a.pack, head = group * a.pack + c % a.pack;
+    const bool used = c < columns;
+    const char* q = used ? static_cast<const char*>(a.q.p) + (b * a.q.outer + token * a.q.middle + head * a.q.head) * 2 : nullptr;
+    s16x8 qf[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) qf[i] = column(q, i, hi, a.d);
+
+    const float* held = nullptr;
+    int position = 0;
+    if constexpr (BIAS) {
+        const int places = bias_places(a.bias.far);
+        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, bias_held + p * places, thread, 256);
+        held = bias_held + (head - group * a.pack) * places;
+        position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
+    }
+
+    f32x16 o[kParts];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) o[i] = f32x16{};
+    float top = -INFINITY, total = 0.f;
+
+    KeyWalk walk;
+    walk.begin(a, b, split * a.tiles_per_split, (split + 1) * a.tiles_per_split);
+    Copier<DP, kKeyTile, 256> ks, vs;
+    ks.init(thread, a.k.middle, a.d);
+    vs.init(thread, a.v.middle, a.d);
+    auto load = [&] {
+        const int valid = walk.count - walk.first;
+        ks.load(thread, static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
+        vs.load(thread, static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
+    };
+    bool more = walk.valid();
+    int now = 0;
+    if (more) {
+        load();
+        ks.store(thread, tile[0][0]);
+        vs.store(thread, tile[0][1]);
+    }
+    __syncthreads();
+    while (more) {
+        const int first = walk.first, left = walk.count - walk.first;
+        walk.next(a);
+        more = walk.valid();
+        if (more) load();
+
+        f32x16 s[2];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            s[sub] = f32x16{};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), qf[i], s[sub]);
+        }
+        bool near = false;
+        float apart = 0.f;
+        if constexpr (BIAS) {
+            const int x0 = first - position;
+            // the wave's tokens lie between its first and last column's
+            const int t0 = __builtin_amdgcn_readfirstlane(position), t1 = __builtin_amdgcn_readlane(position, 31);
+            near = !far_apart(a.bias, first - t1, first + kKeyTile - 1 - t0);
+            if (near) {
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) add_bias<1>(s[sub], a.scale, held, a.bias.far, x0 + 32 * sub + 4 * hi);
+            } else {
+                apart = held[bias_index(a.bias.far, x0)];
+                if (__any(fabsf(apart) > kLargeBias)) {
+#pragma unroll
+                    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) s[sub][r] = __builtin_fmaf(s[sub][r], a.scale, apart);
+                    near = true;
+                }
+            }
+        }
+        if (left < kKeyTile) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * sub + row_of(r, hi) >= left) s[sub][r] = -INFINITY;
+        }
+        // where all keys share one bias s stays the plain product, and scale and bias go into the exponent's one step
+        float most = s[0][0];
+#pragma unroll
+        for (int r = 1; r < 32; ++r) most = fmaxf(most, s[r / 16][r % 16]);
+        most = both_max(most);
+        if (!near && most != -INFINITY) most = __builtin_fmaf(most, a.scale, apart);
+        if (__any(most > top + kSlack)) {
+            const float raised = fmaxf(top, most);
+            const float factor = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - raised) * kLog2e);
+            top = raised;
+            total *= factor;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= factor;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+        const float by = a.scale * kLog2e, shift = (apart - base) * kLog2e;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float x = near ? (s[sub][r] - base) * kLog2e : __builtin_fmaf(s[sub][r], by, shift);
+                s[sub][r] = __builtin_amdgcn_exp2f(x);
+                total += s[sub][r];
+            }
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+            const s16x8 p = rounded<E>(s[step / 2], step % 2);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(tile[now][1], 16 * step, i, lane), p, o[i]);
+        }
+        if (more) {
+            ks.store(thread, tile[now ^ 1][0]);
+            vs.store(thread, tile[now ^ 1][1]);
+        }
+        __syncthreads();
+        now ^= 1;
+    }
+
+    total = both_sum(total);
+    if (!used) return;
+    if (a.splits == 1) {
+        const float factor = total == 0.f ? 0.f : 1.f / total;
+        char* out = static_cast<char*>(a.out.p) + (b * a.out.outer + token * a.out.middle + head * a.out.head) * 2;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const int at = 32 * i + row_of(4 * quad, hi);
+                if (at >= a.d) continue;
+                typename E::T y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = (typename E::T)(o[i][4 * quad + j] * factor);
+                *reinterpret_cast<u32x2*>(out + at * 2) = *reinterpret_cast<u32x2*>(y);
+            }
+        if (a.lse && hi == 0)
+            a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
+    } else {
+        const int64_t at = ((static_cast<int64_t>(split) * a.batch + b) * groups + group) * columns + c;
+        if (hi == 0) a.stat[at] = make_float2(top, total);
+        float* part = a.part + at * a.d;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const int e = 32 * i + row_of(4 * quad, hi);
+                if (e >= a.d) continue;
+                *reinterpret_cast<f32x4*>(part + e) = f32x4{o[i][4 * quad], o[i][4 * quad + 1], o[i][4 * quad + 2], o[i][4 * quad + 3]};
+            }
+    }
+}
+
+template <class E, int DP>
+hipError_t launch_forward(const AttendArgs& a, hipStream_t stream) {
+    const int64_t column_tiles = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns;
+    const int64_t blocks = column_tiles * a.splits * (a.heads / a.pack) * a.batch;
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    const size_t lds = a.bias.table ? a.pack * (2 * a.bias.far + 7) * sizeof(float) : 0;
+    auto kernel = a.bias.table ? forward_kernel<E, DP, true> : forward_kernel<E, DP, false>;
+    kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace vk::attend

@@ -1,0 +1,71 @@
+// What follows the attention kernels where their work was split: the joined softmax of the splits of a row, and the bias
+// table's gradient from the blocks' sums. Both sum in a fixed order.
+#include "attend_tile.hpp"
+
+namespace vk {
+namespace attend {
+
+// One wave per query row: out = sum of exp(top_i - top) part_i / sum of exp(top_i - top) total_i. Two elements a lane.
+template <class E>
+__global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
+    const int lane = threadIdx.x % 64, groups = a.heads / a.pack, columns = a.tokens * a.pack;
+    const int64_t rows = static_cast<int64_t>(a.batch) * groups * columns;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
+    if (row >= rows) return;
+    float top = -INFINITY;
+    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, a.stat[i * rows + row].x);
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f, x = 0.f, y = 0.f;
+    for (int i = 0; i < a.splits; ++i) {
+        const float2 s = a.stat[i * rows + row];
+        const float w = __builtin_amdgcn_exp2f((s.x - base) * kLog2e);
+        total = __builtin_fmaf(w, s.y, total);
+        if (2 * lane < a.d) {
+            const float2 p = *reinterpret_cast<const float2*>(a.part + (i * rows + row) * a.d + 2 * lane);
+            x = __builtin_fmaf(w, p.x, x);
+            y = __builtin_fmaf(w, p.y, y);
+        }
+    }
+    const int c = row % columns, group = row / columns % groups, b = row / columns / groups;
+    const int token = c / a.pack, head = group * a.pack + c % a.pack;
+    const float factor = total == 0.f ? 0.f : 1.f / total;
+    if (2 * lane < a.d) {
+        typename E::T z[2] = {(typename E::T)(x * factor), (typename E::T)(y * factor)};
+        char* out = static_cast<char*>(a.out.p) + (b * a.out.outer + token * a.out.middle + head * a.out.head) * 2;
+        *reinterpret_cast<unsigned*>(out + 4 * lane) = *reinterpret_cast<unsigned*>(z);
+    }
+    if (a.lse && lane == 0)
+        a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
+}
+
+// One wave per (bucket, head).
+template <class E>
+__global__ __launch_bounds__(256) void table_kernel(AttendGradArgs g, int parts) {
+    const int lane = threadIdx.x % 64, at = blockIdx.x * 4 + threadIdx.x / 64;
+    if (at >= g.a.heads * g.a.bias.buckets) return;
+    const int head = at % g.a.heads, bucket = at / g.a.heads;
+    float x = 0.f;
+    for (int i = lane; i < parts; i += 64) x += g.table_part[(static_cast<int64_t>(i) * g.a.heads + head) * g.a.bias.buckets + bucket];
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
+    if (lane == 0) static_cast<typename E::T*>(g.d_table)[at] = (typename E::T)x;
+}
+
+}  // namespace attend
+
+hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.tokens;
+    auto kernel = type == kAttendBf16 ? attend::combine_kernel<attend::Bf16> : attend::combine_kernel<attend::F16>;
+    kernel<<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
+hipError_t launch_attend_grad_table(const AttendGradArgs& g, int type, int parts, hipStream_t stream) {
+    auto kernel = type == kAttendBf16 ? attend::table_kernel<attend::Bf16> : attend::table_kernel<attend::F16>;
+    kernel<<<(g.a.heads * g.a.bias.buckets + 3) / 4, 256, 0, stream>>>(g, parts);
+    return hipGetLastError();
+}
+
+}  // namespace vk

@@ -15,12 +15,11 @@
 #include <string>
 #include <vector>
 
+#include "errors.hpp"
 #include "kernels.hpp"
 #include "planning.hpp"
 #include "slot_order.hpp"
 #include "veckern/veckern.h"
-
-#define VK_EXPORT extern "C" __attribute__((visibility("default")))
 
 namespace vk {
 // Per-m instance tables of the wave-list scan, fp32 (fused_wave_m*.hip) and fp16 tables (fused_wave_h*.hip).
@@ -85,48 +84,12 @@ static __device__ __align__(256) unsigned char scratch[kNoAllocScratchBytes];
 
 namespace {
 
+using vk::fail;
+using vk::Failure;
+using vk::g_error;
+using vk::guarded;
 using vk::Pair;
-
-thread_local std::string g_error;
-
-struct Failure {
-    int code;
-    std::string message;
-};
-
-[[noreturn]] void fail(int code, const std::string& message) { throw Failure{code, message}; }
-
-void require(bool condition, const std::string& message) {
-    if (!condition) fail(VK_ERR_RUNTIME, message);
-}
-
-void hip_check(hipError_t e, const char* what) {
-    if (e != hipSuccess)
-        fail(e == hipErrorOutOfMemory ? VK_ERR_OUT_OF_MEMORY : VK_ERR_DEVICE,
-             std::string(what) + " failed: " + hipGetErrorString(e));
-}
-#define VK_HIP(call) hip_check((call), #call)
-
-template <typename F>
-int guarded(F&& body) {
-    try {
-        body();
-        g_error.clear();
-        return VK_OK;
-    } catch (const Failure& f) {
-        g_error = f.message;
-        return f.code;
-    } catch (const std::bad_alloc&) {
-        g_error = "host allocation failed";
-        return VK_ERR_OUT_OF_MEMORY;
-    } catch (const std::exception& e) {
-        g_error = e.what();
-        return VK_ERR_RUNTIME;
-    } catch (...) {
-        g_error = "unknown error";
-        return VK_ERR_RUNTIME;
-    }
-}
+using vk::require;
 
 template <typename T>
 class DeviceBuffer {
