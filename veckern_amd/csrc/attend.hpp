@@ -10,7 +10,9 @@ namespace vk {
 
 constexpr int kMostEdges = 128;      // bucket edges of a one-sided bias of 256 buckets
 constexpr int kMostDistance = 1024;  // largest max_distance: the bias by distance, and its gradient, are held in LDS
+constexpr int kPad = 15;             // places at either end of the bias by distance (attend_tile.hpp)
 constexpr int kKeyTile = 64;         // keys that a block of the tile kernels holds at once
+constexpr int kFewPassages = 512;    // passages that a block of the few-columns kernel holds the rows of
 constexpr int kColumns = 128;        // query columns of a block of the tile kernels
 
 // A tensor [outer][middle][head][d]: element strides, d contiguous.
@@ -43,6 +45,7 @@ struct AttendArgs {
     float scale = 0.f;            // positive, so that -inf * scale is -inf (0 is taken as 1e-37)
     AttendBias bias;
     // How the work is laid out. pack: query heads of one key head that share a block's columns (column = token * pack + head).
+    // splits: runs of the keys that different blocks take, each of tiles_per_split places of passages x tiles.
     int pack = 1, splits = 1, tiles_per_split = 0;
     float* part = nullptr;   // splits > 1: [splits][batch][heads / pack][tokens * pack][d] unnormalised sums ...
     float2* stat = nullptr;  // ... and [splits][...][tokens * pack] (maximum, sum)
@@ -60,6 +63,7 @@ struct AttendGradArgs {
 enum AttendType { kAttendF16 = 0, kAttendBf16 = 1 };
 
 hipError_t launch_attend_forward(const AttendArgs& a, int type, hipStream_t stream);
+hipError_t launch_attend_few(const AttendArgs& a, int type, hipStream_t stream);
 hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stream);
 // Writes d_q (and delta, and the table's partial sums).
 hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream);

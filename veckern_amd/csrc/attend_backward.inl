@@ -18,22 +18,30 @@ __device__ __forceinline__ void store_four(void* p, int at, const f32x16& x, int
     *reinterpret_cast<u32x2*>(static_cast<char*>(p) + at * 2) = *reinterpret_cast<u32x2*>(y);
 }
 
-// Adds dS of a 32 x 32 tile (lane: one query position) to the sums by distance. Each wave half owns an array, in which its
-// lanes' places differ, and adds to it in program order; lanes beyond the far ends add to a register instead. So no two adds
-// meet whose order is not fixed.
-__device__ __forceinline__ void add_by_distance(const f32x16& ds, float* sums, int far, int x0, float& below, float& above) {
+// Adds dS of a 32 x 32 tile (lane: one query position, x: the distance of the tile's first key from the first query) to a
+// wave's sums by distance, in a fixed order. The tile goes through LDS by diagonals: element (key, query) to row 31 + key -
+// query and place `query` of `skew`, whose other places stay zero; then a lane sums one diagonal and adds it to that distance's
+// place, or, beyond the far ends, to a register. With 36 floats a row neither the writes nor the 16-byte reads share a bank.
+// (Adding each element to its distance's place by an LDS atomic took 130 clocks an instruction.)
+constexpr int kSkew = 36, kSkewFloats = 63 * kSkew;
+__device__ __forceinline__ void add_by_distance(const f32x16& ds, float* skew, float* sums, int far, int x, int lane, float& below,
+                                                float& above) {
+    float* to = skew + (31 - lane % 32 + lane / 32) * kSkew + lane % 32;
 #pragma unroll
-    for (int quad = 0; quad < 4; ++quad) {
-        const int i = x0 + 8 * quad + far + 3;
-        if (i >= 0 && i <= 2 * far + 3) {
+    for (int r = 0; r < 16; ++r) to[tile_row(r, 0) * kSkew] = ds[r];
+    between_lanes();
+    if (lane < 63) {
+        const f32x4* from = reinterpret_cast<const f32x4*>(skew + lane * kSkew);
+        f32x4 y = from[0];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) unsafeAtomicAdd(sums + i + j, ds[4 * quad + j]);
-        } else {
-            const float all = (ds[4 * quad] + ds[4 * quad + 1]) + (ds[4 * quad + 2] + ds[4 * quad + 3]);
-            if (i < 0) below += all;
-            else above += all;
-        }
+        for (int i = 1; i < 8; ++i) y += from[i];
+        const float all = (y[0] + y[1]) + (y[2] + y[3]);
+        const int place = x + lane - 31 + far + kPad;
+        if (place < 0) below += all;
+        else if (place > 2 * far + 2 * kPad) above += all;
+        else sums[place] += all;
     }
+    between_lanes();
 }
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -45,15 +53,15 @@ __device__ __forceinline__ float wave_sum(float x) {
 // The first distance |x| of bucket j of a side.
 __device__ __forceinline__ int bucket_begin(const AttendBias& s, int j) {
     const int exact = s.side / 2;
-    return j <= exact ? j : j - exact - 1 < s.edges ? s.edge[j - exact - 1] : s.far + 4;
+    return j <= exact ? j : j - exact - 1 < s.edges ? s.edge[j - exact - 1] : s.far + kPad + 1;
 }
 
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_q_kernel(AttendGradArgs g) {
     constexpr int kSteps = DP / 16, kParts = DP / 32;
     const AttendArgs& a = g.a;
-    __shared__ s16x8 tile[2][2][kKeyTile * DP / 8];
-    extern __shared__ float shared[];  // the bias by distance, then eight arrays of its gradient's sums
+    __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeyTile>];
+    extern __shared__ float shared[];  // per wave a skewed tile; the bias by distance; per wave its gradient's sums by distance
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
     const int columns = a.tokens * a.pack, column_tiles = (columns + kColumns - 1) / kColumns, groups = a.heads / a.pack;
@@ -67,17 +75,15 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
     const int64_t row = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + token;
-    auto at = [&](const AttendView& v) {
-        return used ? static_cast<char*>(v.p) + (b * v.outer + token * v.middle + head * v.head) * 2 : nullptr;
-    };
+    auto at = [&](const AttendView& v) { return b * v.outer + token * v.middle + head * v.head; };
     s16x8 qf[kSteps], df[kSteps];
     float delta = 0.f;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-        qf[i] = column(at(a.q), i, hi, a.d);
-        df[i] = column(at(g.d_out), i, hi, a.d);
+        qf[i] = column(a.q, at(a.q), used, i, hi, a.d);
+        df[i] = column(g.d_out, at(g.d_out), used, i, hi, a.d);
         const auto x = __builtin_bit_cast(typename E::x8, df[i]);
-        const auto y = __builtin_bit_cast(typename E::x8, column(at(a.out), i, hi, a.d));
+        const auto y = __builtin_bit_cast(typename E::x8, column(a.out, at(a.out), used, i, hi, a.d));
 #pragma unroll
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(x[j]), static_cast<float>(y[j]), delta);
     }
@@ -90,12 +96,15 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     const float scale_log2 = a.scale * kLog2e;
     int position = 0;
     float below = 0.f, above = 0.f;
-    float* sums = nullptr;
+    float *held = nullptr, *sums = nullptr, *skew = nullptr;
     if constexpr (BIAS) {
         const int places = bias_places(a.bias.far);
-        fill_bias<E>(a.bias, head, shared, thread, 256);
-        for (int i = thread; i < 8 * places; i += 256) shared[places + i] = 0.f;
-        sums = shared + (1 + 2 * wave + hi) * places;
+        skew = shared + wave * kSkewFloats;
+        held = shared + 4 * kSkewFloats;
+        sums = held + (1 + wave) * places;
+        fill_bias<E>(a.bias, head, held, thread, 256);
+        for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
+        for (int i = thread; i < 4 * places; i += 256) held[places + i] = 0.f;
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
 
@@ -110,120 +119,142 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     vs.init(thread, a.v.middle, a.d);
     auto load = [&] {
         const int valid = walk.count - walk.first;
-        ks.load(thread, static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
-        vs.load(thread, static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
+        ks.load(static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
+        vs.load(static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
     };
     bool more = walk.valid();
     int now = 0;
     if (more) {
         load();
-        ks.store(thread, tile[0][0]);
-        vs.store(thread, tile[0][1]);
+        ks.store(tile[0][0]);
+        vs.store(tile[0][1]);
     }
     __syncthreads();
+    const char *k, *v;
+    auto products = [&](f32x16& s, f32x16& dp, int sub) {
+        s = dp = f32x16{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) dp = E::mfma(straight<DP>(v, 32 * sub, i, lane), df[i], dp);
+    };
+    auto gather = [&](const f32x16& ds, int sub) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const s16x8 x = rounded<E>(ds, half);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 32 * sub + 16 * half, i, lane), x, dq[i]);
+        }
+    };
     while (more) {
         const int first = walk.first, left = walk.count - walk.first;
         walk.next(a);
         more = walk.valid();
         if (more) load();
-        bool near = false, wide = false;
+        k = tile[now][0];
+        v = tile[now][1];
+        bool plain = left >= kKeyTile;  // all keys are there, and share one bias
         float apart = 0.f;
+        int t0 = 0;
         if constexpr (BIAS) {
-            const int t0 = __builtin_amdgcn_readfirstlane(position), t1 = __builtin_amdgcn_readlane(position, 31);
-            near = !far_apart(a.bias, first - t1, first + kKeyTile - 1 - t0);
-            if (!near) {
-                apart = shared[bias_index(a.bias.far, first - position)];
-                wide = __any(fabsf(apart) > kLargeBias);
-            }
+            t0 = __builtin_amdgcn_readfirstlane(position);
+            apart = held[bias_index(a.bias.far, first - position)];
+            plain = plain && far_apart(a.bias, first - (t0 + 31), first + kKeyTile - 1 - t0) && !__any(fabsf(apart) > kLargeBias);
         }
+        f32x16 s[2], dp[2];
+        if (plain) {
+            const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
+            auto weights = [&](f32x16& s, const f32x16& dp) {
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            f32x16 s{}, dp{};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), qf[i], s);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) dp = E::mfma(straight<DP>(tile[now][1], 32 * sub, i, lane), df[i], dp);
-            const int x0 = first + 32 * sub + 4 * hi - position;
-            if (BIAS && near) {
-                add_bias<1>(s, a.scale, shared, a.bias.far, x0);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r] - lse.x, kLog2e, lse.y);
-            } else if (BIAS && wide) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(__builtin_fmaf(s[r], a.scale, apart) - lse.x, kLog2e, lse.y);
-            } else {
-                const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], scale_log2, shift);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float p = __builtin_amdgcn_exp2f(s[r]);
-                if (left < kKeyTile && 32 * sub + row_of(r, hi) >= left) p = 0.f;
-                s[r] = p * (dp[r] - delta);
-            }
+                for (int r = 0; r < 16; ++r)
+                    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, shift)) * (dp[r] - delta);
+            };
+            // the two halves of the tile one step apart: the weights of one are taken beside the products of the other
+            between_runs();
+            products(s[0], dp[0], 0);
+            feed<2 * kSteps, 1, 4>();
+            between_runs();
+            products(s[1], dp[1], 1);
+            weights(s[0], dp[0]);
+            feed<2 * kSteps, 1, 4, 64 / kSteps>();
+            between_runs();
+            gather(s[0], 0);
+            weights(s[1], dp[1]);
+            feed<2 * kParts, 2, 2, 128 / kSteps>();
+            between_runs();
+            gather(s[1], 1);
+            feed<2 * kParts, 2, 3>();
+            between_runs();
             if constexpr (BIAS) {
-                if (near) {
-                    add_by_distance(s, sums, a.bias.far, x0, below, above);
-                } else {
-                    float all = 0.f;
+                float all = 0.f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) all += s[r];
-                    if (first < position) below += all;
-                    else above += all;
-                }
+                for (int r = 0; r < 32; ++r) all += s[r / 16][r % 16];
+                if (first < position) below += all;
+                else above += all;
             }
+        } else {
 #pragma unroll
-            for (int step = 0; step < 2; ++step) {
-                const s16x8 x = rounded<E>(s, step);
+            for (int sub = 0; sub < 2; ++sub) {
+                products(s[sub], dp[sub], sub);
+                f32x16& x = s[sub];
+                if constexpr (BIAS) {
+                    add_bias<1>(x, a.scale, held, a.bias.far, first + 32 * sub + hi - position);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kParts; ++i)
-                    dq[i] = E::mfma(transposed<DP>(tile[now][0], 32 * sub + 16 * step, i, lane), x, dq[i]);
+                    for (int r = 0; r < 16; ++r) x[r] *= a.scale;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - lse.x, kLog2e, lse.y));
+                    x[r] = 32 * sub + tile_row(r, hi) < left ? p * (dp[sub][r] - delta) : 0.f;
+                }
+                if constexpr (BIAS) add_by_distance(x, skew, sums, a.bias.far, first + 32 * sub - t0, lane, below, above);
+                gather(x, sub);
             }
         }
         if (more) {
-            ks.store(thread, tile[now ^ 1][0]);
-            vs.store(thread, tile[now ^ 1][1]);
+            ks.store(tile[now ^ 1][0]);
+            vs.store(tile[now ^ 1][1]);
         }
         __syncthreads();
         now ^= 1;
     }
 
     if (used) {
-        char* out = at(g.d_q);
+        char* out = static_cast<char*>(g.d_q.p) + at(g.d_q) * 2;
 #pragma unroll
         for (int i = 0; i < kParts; ++i)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
-                const int e = 32 * i + row_of(4 * quad, hi);
+                const int e = 32 * i + mfma_row(4 * quad, hi);
                 if (e < a.d) store_four<typename E::T>(out, e, dq[i], quad, g.scale);
             }
     }
     if constexpr (BIAS) {
         const AttendBias& s = a.bias;
-        const int places = bias_places(s.far);
+        const int places = bias_places(s.far), zero = s.far + kPad;  // the place of distance 0
         below = wave_sum(below);
         above = wave_sum(above);
-        if (lane == 0) {  // this wave's lower array; its own adds came before
+        if (lane == 0) {
             sums[0] += below;
             sums[places - 1] += above;
         }
         __syncthreads();
         for (int i = thread; i < places; i += 256) {
             float x = 0.f;
-            for (int w = 1; w <= 8; ++w) x += shared[w * places + i];
-            shared[i] = x;
+            for (int w = 1; w <= 4; ++w) x += held[w * places + i];
+            held[i] = x;
         }
         __syncthreads();
         for (int bucket = thread; bucket < s.buckets; bucket += 256) {
-            const int j = bucket % s.side, from = bucket_begin(s, j), to = j + 1 < s.side ? bucket_begin(s, j + 1) : s.far + 4;
+            const int j = bucket % s.side, from = bucket_begin(s, j), to = j + 1 < s.side ? bucket_begin(s, j + 1) : zero + 1;
             float x = 0.f;
             if (bucket < s.side) {
-                for (int y = from; y < to; ++y) x += shared[s.far + 3 - y];
+                for (int y = from; y < to; ++y) x += held[zero - y];
                 if (!s.two_sided && j == 0)
-                    for (int y = 1; y <= s.far + 3; ++y) x += shared[s.far + 3 + y];
+                    for (int y = 1; y <= zero; ++y) x += held[zero + y];
             } else {
-                for (int y = max(from, 1); y < to; ++y) x += shared[s.far + 3 + y];
+                for (int y = max(from, 1); y < to; ++y) x += held[zero + y];
             }
             g.table_part[((static_cast<int64_t>(b) * column_tiles + column_tile) * a.heads + head) * s.buckets + bucket] = x;
         }
@@ -232,11 +263,12 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
 
 // One block: 128 keys of a bank row and key head, each wave 32 of them; walks the request's query tiles, head by head.
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_kv_kernel(AttendGradArgs g) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = 64;
     const AttendArgs& a = g.a;
-    __shared__ s16x8 tile[2][2][kQueries * DP / 8];
-    // of each query: lse and -what its rounding left off * log2(e); both as one in log2 units, negative; delta
+    __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kQueries>];
+    // of each query, in the order of the products' rows: lse and -what its rounding left off * log2(e); both as one in log2
+    // units, negative; delta
     __shared__ __align__(16) float stat[2][4][kQueries];
     extern __shared__ float bias_held[];
 
@@ -258,12 +290,12 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
     if (key_tile * kColumns < count) {
         s16x8 kf[kSteps], vf[kSteps];
         {
-            const char* k = there ? static_cast<const char*>(a.k.p) + (row * a.k.outer + key * a.k.middle + kv_head * a.k.head) * 2 : nullptr;
-            const char* v = there ? static_cast<const char*>(a.v.p) + (row * a.v.outer + key * a.v.middle + kv_head * a.v.head) * 2 : nullptr;
+            const int64_t k = row * a.k.outer + key * a.k.middle + kv_head * a.k.head;
+            const int64_t v = row * a.v.outer + key * a.v.middle + kv_head * a.v.head;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                kf[i] = column(k, i, hi, a.d);
-                vf[i] = column(v, i, hi, a.d);
+                kf[i] = column(a.k, k, there, i, hi, a.d);
+                vf[i] = column(a.v, v, there, i, hi, a.d);
             }
         }
         const float scale_log2 = a.scale * kLog2e;
@@ -276,8 +308,8 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
         int head = kv_head * share, first = 0;
         auto load = [&] {
             const int valid = a.tokens - first;
-            qs.load(thread, static_cast<const char*>(a.q.p) + (b * a.q.outer + first * a.q.middle + head * a.q.head) * 2, valid);
-            ds.load(thread, static_cast<const char*>(g.d_out.p) + (b * g.d_out.outer + first * g.d_out.middle + head * g.d_out.head) * 2, valid);
+            qs.load(static_cast<const char*>(a.q.p) + (b * a.q.outer + first * a.q.middle + head * a.q.head) * 2, valid);
+            ds.load(static_cast<const char*>(g.d_out.p) + (b * g.d_out.outer + first * g.d_out.middle + head * g.d_out.head) * 2, valid);
             if (thread < kQueries) {
                 const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + first + thread;
                 lse = thread < valid ? a.lse[at] : make_float2(-INFINITY, 0.f);
@@ -286,13 +318,14 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
             }
         };
         auto store = [&](int to) {
-            qs.store(thread, tile[to][0]);
-            ds.store(thread, tile[to][1]);
+            qs.store(tile[to][0]);
+            ds.store(tile[to][1]);
             if (thread < kQueries) {
-                stat[to][0][thread] = lse.x;
-                stat[to][1][thread] = lse.y;
-                stat[to][2][thread] = __builtin_fmaf(lse.x, -kLog2e, lse.y);
-                stat[to][3][thread] = delta;
+                const int at = place_of(thread);
+                stat[to][0][at] = lse.x;
+                stat[to][1][at] = lse.y;
+                stat[to][2][at] = __builtin_fmaf(lse.x, -kLog2e, lse.y);
+                stat[to][3][at] = delta;
             }
         };
         load();
@@ -301,6 +334,35 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
         __syncthreads();
         int now = 0;
         bool more = true;
+        const char *q, *d;
+        auto of = [&](int which, int sub, int quad) {
+            return *reinterpret_cast<const f32x4*>(&stat[now][which][32 * sub + mfma_row(4 * quad, hi)]);
+        };
+        auto products = [&](f32x16& s, f32x16& dp, int sub) {
+            s = dp = f32x16{};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(q, 32 * sub, i, lane), kf[i], s);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) dp = E::mfma(straight<DP>(d, 32 * sub, i, lane), vf[i], dp);
+        };
+        auto times_rest = [&](const f32x16& p, f32x16& dp, int sub) {
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const f32x4 e = of(3, sub, quad);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[4 * quad + j] = p[4 * quad + j] * (dp[4 * quad + j] - e[j]);
+            }
+        };
+        auto gather = [&](const f32x16& p, const f32x16& ds, int sub) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const s16x8 x = rounded<E>(p, half), y = rounded<E>(ds, half);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) dv[i] = E::mfma(transposed<DP>(d, 32 * sub + 16 * half, i, lane), x, dv[i]);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) dk[i] = E::mfma(transposed<DP>(q, 32 * sub + 16 * half, i, lane), y, dk[i]);
+            }
+        };
         while (more) {
             const int from = first;
             first += kQueries;
@@ -312,55 +374,61 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
             }
             more = head < (kv_head + 1) * share;
             if (more) load();
-            bool near = false;
+            q = tile[now][0];
+            d = tile[now][1];
+            bool plain = true;  // all places share one bias
             float apart = 0.f;
-            bool wide = false;
             if constexpr (BIAS) {
                 const int k0 = key_tile * kColumns + wave * 32;
-                near = !far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start));
-                if (!near) {
-                    apart = bias_held[bias_index(a.bias.far, key - (from + start))];
-                    wide = __any(fabsf(apart) > kLargeBias);
-                }
+                apart = bias_held[bias_index(a.bias.far, key - (from + start))];
+                plain = far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start)) &&
+                        !__any(fabsf(apart) > kLargeBias);
             }
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                f32x16 s{}, dp{};
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), kf[i], s);
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) dp = E::mfma(straight<DP>(tile[now][1], 32 * sub, i, lane), vf[i], dp);
-                if (BIAS && near) {
-                    add_bias<-1>(s, a.scale, bias_held, a.bias.far, key - (from + start + 32 * sub + 4 * hi));
-                } else if (BIAS && wide) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], a.scale, apart);
-                }
-                const bool added = BIAS && (near || wide);
+            f32x16 s[2], dp[2];
+            if (plain) {
                 const float apart_log2 = apart * kLog2e;
+                auto weights = [&](f32x16& s, f32x16& dp, int sub) {
 #pragma unroll
-                for (int quad = 0; quad < 4; ++quad) {
-                    const f32x4 l = *reinterpret_cast<const f32x4*>(&stat[now][0][32 * sub + row_of(4 * quad, hi)]);
-                    const f32x4 low = *reinterpret_cast<const f32x4*>(&stat[now][1][32 * sub + row_of(4 * quad, hi)]);
-                    const f32x4 one = *reinterpret_cast<const f32x4*>(&stat[now][2][32 * sub + row_of(4 * quad, hi)]);
-                    const f32x4 e = *reinterpret_cast<const f32x4*>(&stat[now][3][32 * sub + row_of(4 * quad, hi)]);
+                    for (int quad = 0; quad < 4; ++quad) {
+                        const f32x4 one = of(2, sub, quad);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * quad + j;
-                        const float x = added ? __builtin_fmaf(s[r] - l[j], kLog2e, low[j])
-                                              : __builtin_fmaf(s[r], scale_log2, BIAS ? apart_log2 + one[j] : one[j]);
-                        s[r] = there ? __builtin_amdgcn_exp2f(x) : 0.f;
-                        dp[r] = s[r] * (dp[r] - e[j]);
+                        for (int j = 0; j < 4; ++j)
+                            s[4 * quad + j] = __builtin_amdgcn_exp2f(
+                                __builtin_fmaf(s[4 * quad + j], scale_log2, BIAS ? apart_log2 + one[j] : one[j]));
                     }
-                }
+                    times_rest(s, dp, sub);
+                };
+                // the two halves of the tile one step apart: the weights of one are taken beside the products of the other
+                between_runs();
+                products(s[0], dp[0], 0);
+                feed<2 * kSteps, 1, 4>();
+                between_runs();
+                products(s[1], dp[1], 1);
+                weights(s[0], dp[0], 0);
+                feed<2 * kSteps, 1, 4, 64 / kSteps>();
+                between_runs();
+                gather(s[0], dp[0], 0);
+                weights(s[1], dp[1], 1);
+                feed<4 * kParts, 2, 2, 64 / kSteps>();
+                between_runs();
+                gather(s[1], dp[1], 1);
+                feed<4 * kParts, 2, 3>();
+                between_runs();
+            } else {
 #pragma unroll
-                for (int step = 0; step < 2; ++step) {
-                    const s16x8 p = rounded<E>(s, step), x = rounded<E>(dp, step);
+                for (int sub = 0; sub < 2; ++sub) {
+                    products(s[sub], dp[sub], sub);
+                    f32x16& x = s[sub];
+                    add_bias<-1>(x, a.scale, bias_held, a.bias.far, key - (from + start + 32 * sub + hi));
 #pragma unroll
-                    for (int i = 0; i < kParts; ++i) {
-                        dv[i] = E::mfma(transposed<DP>(tile[now][1], 32 * sub + 16 * step, i, lane), p, dv[i]);
-                        dk[i] = E::mfma(transposed<DP>(tile[now][0], 32 * sub + 16 * step, i, lane), x, dk[i]);
+                    for (int quad = 0; quad < 4; ++quad) {
+                        const f32x4 l = of(0, sub, quad), low = of(1, sub, quad);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            x[4 * quad + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[4 * quad + j] - l[j], kLog2e, low[j]));
                     }
+                    times_rest(x, dp[sub], sub);
+                    gather(x, dp[sub], sub);
                 }
             }
             if (more) store(now ^ 1);
@@ -382,7 +450,7 @@ __global__ __launch_bounds__(256, 1) void grad_kv_kernel(AttendGradArgs g) {
         for (int i = 0; i < kParts; ++i)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
-                const int e = 32 * i + row_of(4 * quad, hi);
+                const int e = 32 * i + mfma_row(4 * quad, hi);
                 if (e >= a.d) continue;
                 const f32x16 zero{};
                 store_four<typename E::T>(k, e, there ? dk[i] : zero, quad, g.scale);
@@ -396,7 +464,7 @@ hipError_t launch_grad_q(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns * (a.heads / a.pack) * a.batch;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const size_t lds = a.bias.table ? 9 * (2 * a.bias.far + 7) * sizeof(float) : 0;
+    const size_t lds = a.bias.table ? (4 * kSkewFloats + 5 * (2 * a.bias.far + 2 * kPad + 1)) * sizeof(float) : 0;
     auto kernel = a.bias.table ? grad_q_kernel<E, DP, true> : grad_q_kernel<E, DP, false>;
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
     return hipGetLastError();
@@ -407,7 +475,7 @@ hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t blocks = static_cast<int64_t>((a.length + kColumns - 1) / kColumns) * a.kv_heads * a.bank;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const size_t lds = a.bias.table ? (2 * a.bias.far + 7) * sizeof(float) : 0;
+    const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     auto kernel = a.bias.table ? grad_kv_kernel<E, DP, true> : grad_kv_kernel<E, DP, false>;
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
     return hipGetLastError();

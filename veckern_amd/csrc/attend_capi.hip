@@ -10,6 +10,7 @@ namespace vk {
 
 #define VK_ATTEND_INSTANCES(type, size)                                              \
     hipError_t attend_forward_##type##_##size(const AttendArgs& a, hipStream_t stream);     \
+    hipError_t attend_few_##type##_##size(const AttendArgs& a, hipStream_t stream);         \
     hipError_t attend_grad_q_##type##_##size(const AttendGradArgs& g, hipStream_t stream);  \
     hipError_t attend_grad_kv_##type##_##size(const AttendGradArgs& g, hipStream_t stream);
 VK_ATTEND_INSTANCES(bf16, 64)
@@ -20,6 +21,10 @@ VK_ATTEND_INSTANCES(f16, 128)
 hipError_t launch_attend_forward(const AttendArgs& a, int type, hipStream_t stream) {
     if (type == kAttendBf16) return a.d <= 64 ? attend_forward_bf16_64(a, stream) : attend_forward_bf16_128(a, stream);
     return a.d <= 64 ? attend_forward_f16_64(a, stream) : attend_forward_f16_128(a, stream);
+}
+hipError_t launch_attend_few(const AttendArgs& a, int type, hipStream_t stream) {
+    if (type == kAttendBf16) return a.d <= 64 ? attend_few_bf16_64(a, stream) : attend_few_bf16_128(a, stream);
+    return a.d <= 64 ? attend_few_f16_64(a, stream) : attend_few_f16_128(a, stream);
 }
 hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream) {
     if (type == kAttendBf16) return g.a.d <= 64 ? attend_grad_q_bf16_64(g, stream) : attend_grad_q_bf16_128(g, stream);
@@ -143,21 +148,31 @@ AttendArgs args_of(const vk_attention* x, bool tensors) {
     return a;
 }
 
-// Blocks that fill the card's 256 CUs twice: below that the keys are split.
-constexpr int64_t kEnoughBlocks = 512;
+constexpr int64_t kUnits = 256;  // compute units of the card
+
+// Whether a call has so few columns for each key head that its time is the reading of the states.
+bool few_columns(const AttendArgs& a) { return static_cast<int64_t>(a.tokens) * a.pack <= 32; }
+
+// Splits the keys into runs of whole tiles until there are about `wanted` blocks, none with less than `least` tiles.
+void split_keys(AttendArgs& a, int tile, int64_t blocks, int64_t wanted, int least, int most_tiles) {
+    const int tiles = (a.length + tile - 1) / tile * a.passages;
+    int64_t splits = 1;
+    if (blocks > 0 && blocks < wanted) splits = std::min<int64_t>((wanted + blocks - 1) / blocks, tiles / least);
+    splits = std::max<int64_t>({splits, 1, (tiles + most_tiles - 1) / most_tiles});
+    a.tiles_per_split = static_cast<int>((tiles + splits - 1) / splits);
+    a.splits = a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
+}
 
 void plan_forward(AttendArgs& a) {
     const int share = a.heads / a.kv_heads;
     a.pack = share;
-    if (a.bias.table && static_cast<size_t>(share) * (2 * a.bias.far + 7) * sizeof(float) > 16384) a.pack = 1;
-    const int tiles = (a.length + vk::kKeyTile - 1) / vk::kKeyTile * a.passages;
-    const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + vk::kColumns - 1) / vk::kColumns * (a.heads / a.pack) * a.batch;
-    a.splits = 1;
-    a.tiles_per_split = tiles;
-    if (blocks > 0 && blocks < kEnoughBlocks && tiles > 1) {
-        const int64_t wanted = std::min<int64_t>((kEnoughBlocks + blocks - 1) / blocks, tiles);
-        a.tiles_per_split = static_cast<int>((tiles + wanted - 1) / wanted);
-        a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+    if (a.bias.table && static_cast<size_t>(share) * (2 * a.bias.far + 2 * vk::kPad + 1) * sizeof(float) > 16384) a.pack = 1;
+    const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
+    if (few_columns(a)) {
+        const int per_row = (a.length + 31) / 32;  // a run of tiles touches one passage more than it fills
+        split_keys(a, 32, rest, kUnits, 32, std::max(1, (vk::kFewPassages - 1) * std::max(per_row, 1)));
+    } else {
+        split_keys(a, vk::kKeyTile, (columns + vk::kColumns - 1) / vk::kColumns * rest, 2 * kUnits, 1, 1 << 30);
     }
 }
 size_t query_rows(const AttendArgs& a) { return static_cast<size_t>(a.batch) * a.heads * a.tokens; }
@@ -214,7 +229,7 @@ VK_EXPORT int vk_attend(const vk_attention* x, void* workspace, size_t workspace
             a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) + align(a.splits * query_rows(a) * a.d * sizeof(float)));
         }
         const auto on = static_cast<hipStream_t>(stream);
-        VK_HIP(vk::launch_attend_forward(a, x->type, on));
+        VK_HIP(few_columns(a) ? vk::launch_attend_few(a, x->type, on) : vk::launch_attend_forward(a, x->type, on));
         if (a.splits > 1) VK_HIP(vk::launch_attend_combine(a, x->type, on));
     });
 }

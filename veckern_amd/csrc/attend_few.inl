@@ -1,0 +1,206 @@
+// The forward pass for few query columns (a new token, or a few, with the query heads that share a key head): what it takes is
+// reading the states once. A block holds up to 32 columns; its eight waves walk the key tiles (32 rows) in turn, each with its
+// own columns' maxima, sums and outputs, which are joined in LDS at the end, so most calls are one launch and few blocks keep
+// many loads in flight: a wave has its next tile's K and V (16 KB at 128 elements a head) under way while it works on one. Nothing
+// waits at a barrier in between. Products, roundings and the raised maximum are those of the tile kernel (attend_forward.inl).
+#include "attend_tile.hpp"
+
+namespace vk::attend {
+
+constexpr int kFewWaves = 8, kFewKeys = 32;
+
+template <int DP>
+constexpr int kFewTiles = kFewWaves * 2 * kTileBytes<DP, kFewKeys>;
+static_assert(kFewWaves * 32 * (64 + 4) * 4 <= kFewTiles<64> && kFewWaves * 32 * (128 + 4) * 4 <= kFewTiles<128>,
+              "the waves' outputs are joined where the tiles were");
+
+template <class E, int DP, bool BIAS>
+__global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(AttendArgs a) {
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kThreads = 64 * kFewWaves;
+    extern __shared__ __align__(16) char shared[];  // tiles of each wave; (row, positions) of the passages; the bias by distance
+    const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64), hi = lane / 32;
+    const int columns = a.tokens * a.pack, column_tiles = (columns + 31) / 32, groups = a.heads / a.pack;
+    int place = xcd_place(blockIdx.x, gridDim.x);
+    const int column_tile = place % column_tiles;
+    place /= column_tiles;
+    const int split = place % a.splits;
+    place /= a.splits;
+    const int group = place % groups, b = place / groups;
+    const int kv_head = group * a.pack / (a.heads / a.kv_heads);
+
+    const int per_row = (a.length + kFewKeys - 1) / kFewKeys;
+    const int begin = split * a.tiles_per_split, end = min(begin + a.tiles_per_split, per_row * a.passages);
+    char* mine = shared + wave * 2 * kTileBytes<DP, kFewKeys>;
+    int2* found = reinterpret_cast<int2*>(shared + kFewTiles<DP>);
+    const int r0 = per_row ? begin / per_row : 0;
+    if (begin < end) {
+        for (int r = r0 + thread; r <= (end - 1) / per_row; r += kThreads) {
+            int row = b * a.passages + r, count = a.length;
+            if (a.rows) row = a.rows[b * a.rows_outer + r * a.rows_step];
+            if (a.rows && (row < 0 || row >= a.bank)) count = 0;
+            else if (a.lengths) count = min(max(a.lengths[row], 0), a.length);
+            found[r - r0] = make_int2(row, count);
+        }
+    }
+
+    const int c = column_tile * 32 + lane % 32;
+    const int token = c / a.pack, head = group * a.pack + c % a.pack;
+    const bool used = c < columns;
+    const int64_t q = b * a.q.outer + token * a.q.middle + head * a.q.head;
+    s16x8 qf[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
+    const float* held = nullptr;
+    int position = 0;
+    if constexpr (BIAS) {
+        float* all = reinterpret_cast<float*>(shared + kFewTiles<DP> + kFewPassages * sizeof(int2));
+        const int places = bias_places(a.bias.far);
+        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, all + p * places, thread, kThreads);
+        held = all + (head - group * a.pack) * places;
+        position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
+    }
+    __syncthreads();
+
+    f32x16 o[kParts];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) o[i] = f32x16{};
+    float top = -INFINITY, total = 0.f;
+
+    Copier<DP, kFewKeys, 64> ks, vs;
+    ks.init(lane, a.k.middle, a.d);
+    vs.init(lane, a.v.middle, a.d);
+    int at = begin + wave, r = at / max(per_row, 1), tile = at - r * per_row, first = 0, left = 0;
+    // goes on to the wave's next tile with a key, and sets its loads going
+    auto load = [&] {
+        for (; at < end; at += kFewWaves, tile += kFewWaves) {
+            while (tile >= per_row) {
+                tile -= per_row;
+                ++r;
+            }
+            const int2 x = found[r - r0];
+            first = tile * kFewKeys;
+            left = uniform(x.y) - first;
+            if (left <= 0) continue;
+            const int64_t row = uniform(x.x);
+            ks.load(static_cast<const char*>(a.k.p) + (row * a.k.outer + first * a.k.middle + kv_head * a.k.head) * 2, left);
+            vs.load(static_cast<const char*>(a.v.p) + (row * a.v.outer + first * a.v.middle + kv_head * a.v.head) * 2, left);
+            at += kFewWaves;
+            tile += kFewWaves;
+            return true;
+        }
+        return false;
+    };
+    bool more = load();
+    while (more) {
+        ks.store(mine);
+        vs.store(mine + kTileBytes<DP, kFewKeys>);
+        between_lanes();
+        const int from = first, there = left;
+        more = load();
+
+        f32x16 s{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(mine, 0, i, lane), qf[i], s);
+        if constexpr (BIAS) {
+            add_bias<1>(s, a.scale, held, a.bias.far, from - position + hi);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] *= a.scale;
+        }
+        if (there < kFewKeys) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (tile_row(i, hi) >= there) s[i] = -INFINITY;
+        }
+        float most = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[i]);
+        most = both_max(most);
+        if (__any(most > top + kSlack)) {
+            const float raised = fmaxf(top, most);
+            const float factor = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - raised) * kLog2e);
+            top = raised;
+            total *= factor;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[i][j] *= factor;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f((s[i] - base) * kLog2e);
+            total += s[i];
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const s16x8 p = rounded<E>(s, half);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i)
+                o[i] = E::mfma(transposed<DP>(mine + kTileBytes<DP, kFewKeys>, 16 * half, i, lane), p, o[i]);
+        }
+        between_lanes();
+    }
+
+    // the waves' parts, joined
+    constexpr int kRow = DP + 4;
+    float* parts = reinterpret_cast<float*>(shared);
+    float2* stats = reinterpret_cast<float2*>(found);
+    total = both_sum(total);
+    __syncthreads();
+    if (used) {
+        float* to = parts + (wave * 32 + lane % 32) * kRow;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad)
+                *reinterpret_cast<f32x4*>(to + 32 * i + mfma_row(4 * quad, hi)) =
+                    f32x4{o[i][4 * quad], o[i][4 * quad + 1], o[i][4 * quad + 2], o[i][4 * quad + 3]};
+        if (hi == 0) stats[wave * 32 + lane] = make_float2(top, total);
+    }
+    __syncthreads();
+    const int here = min(columns - column_tile * 32, 32), quads = a.d / 4;
+    for (int i = thread; i < here * quads; i += kThreads) {
+        const int x = i / quads, e = i % quads * 4;
+        float most = -INFINITY, sum = 0.f;
+        for (int w = 0; w < kFewWaves; ++w) most = fmaxf(most, stats[w * 32 + x].x);
+        const float base = most == -INFINITY ? 0.f : most;
+        f32x4 y{};
+        for (int w = 0; w < kFewWaves; ++w) {
+            const float2 s = stats[w * 32 + x];
+            const float weight = __builtin_amdgcn_exp2f((s.x - base) * kLog2e);
+            sum = __builtin_fmaf(weight, s.y, sum);
+            y += weight * *reinterpret_cast<const f32x4*>(parts + (w * 32 + x) * kRow + e);
+        }
+        const int column = column_tile * 32 + x, t = column / a.pack, h = group * a.pack + column % a.pack;
+        if (a.splits == 1) {
+            const float factor = sum == 0.f ? 0.f : 1.f / sum;
+            typename E::T z[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[j] = (typename E::T)(y[j] * factor);
+            char* out = static_cast<char*>(a.out.p) + (b * a.out.outer + t * a.out.middle + h * a.out.head + e) * 2;
+            *reinterpret_cast<u32x2*>(out) = *reinterpret_cast<u32x2*>(z);
+            if (a.lse && e == 0) a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.tokens + t] = logarithm(most, sum);
+        } else {
+            const int64_t at = ((static_cast<int64_t>(split) * a.batch + b) * groups + group) * columns + column;
+            if (e == 0) a.stat[at] = make_float2(most, sum);
+            *reinterpret_cast<f32x4*>(a.part + at * a.d + e) = y;
+        }
+    }
+}
+
+template <class E, int DP>
+hipError_t launch_few(const AttendArgs& a, hipStream_t stream) {
+    const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + 31) / 32 * a.splits * (a.heads / a.pack) * a.batch;
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    const size_t lds = kFewTiles<DP> + kFewPassages * sizeof(int2) +
+                       (a.bias.table ? a.pack * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0);
+    auto kernel = a.bias.table ? few_kernel<E, DP, true> : few_kernel<E, DP, false>;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(lds));
+    if (e != hipSuccess) return e;
+    kernel<<<static_cast<unsigned>(blocks), 64 * kFewWaves, lds, stream>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace vk::attend

@@ -1,0 +1,6 @@
+// Few-columns forward kernels for bf16 inputs and head sizes up to 128.
+#include "attend_few.inl"
+
+namespace vk {
+hipError_t attend_few_bf16_128(const AttendArgs& a, hipStream_t stream) { return attend::launch_few<attend::Bf16, 128>(a, stream); }
+}  // namespace vk

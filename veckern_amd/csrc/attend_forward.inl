@@ -13,12 +13,10 @@
 
 namespace vk::attend {
 
-constexpr float kSlack = 5.f;
-
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendArgs a) {
     constexpr int kSteps = DP / 16, kParts = DP / 32;
-    __shared__ s16x8 tile[2][2][kKeyTile * DP / 8];
+    __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeyTile>];
     extern __shared__ float bias_held[];
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
@@ -34,10 +32,10 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
     const int c = column_tile * kColumns + wave * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
-    const char* q = used ? static_cast<const char*>(a.q.p) + (b * a.q.outer + token * a.q.middle + head * a.q.head) * 2 : nullptr;
+    const int64_t q = b * a.q.outer + token * a.q.middle + head * a.q.head;
     s16x8 qf[kSteps];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) qf[i] = column(q, i, hi, a.d);
+    for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
 
     const float* held = nullptr;
     int position = 0;
@@ -60,15 +58,15 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
     vs.init(thread, a.v.middle, a.d);
     auto load = [&] {
         const int valid = walk.count - walk.first;
-        ks.load(thread, static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
-        vs.load(thread, static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
+        ks.load(static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
+        vs.load(static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
     };
     bool more = walk.valid();
     int now = 0;
     if (more) {
         load();
-        ks.store(thread, tile[0][0]);
-        vs.store(thread, tile[0][1]);
+        ks.store(tile[0][0]);
+        vs.store(tile[0][1]);
     }
     __syncthreads();
     while (more) {
@@ -84,6 +82,8 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), qf[i], s[sub]);
         }
+        feed<2 * kSteps, 1, 4>();
+        __builtin_amdgcn_sched_barrier(0);
         bool near = false;
         float apart = 0.f;
         if constexpr (BIAS) {
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
             near = !far_apart(a.bias, first - t1, first + kKeyTile - 1 - t0);
             if (near) {
 #pragma unroll
-                for (int sub = 0; sub < 2; ++sub) add_bias<1>(s[sub], a.scale, held, a.bias.far, x0 + 32 * sub + 4 * hi);
+                for (int sub = 0; sub < 2; ++sub) add_bias<1>(s[sub], a.scale, held, a.bias.far, x0 + 32 * sub + hi);
             } else {
                 apart = held[bias_index(a.bias.far, x0)];
                 if (__any(fabsf(apart) > kLargeBias)) {
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
             for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (32 * sub + row_of(r, hi) >= left) s[sub][r] = -INFINITY;
+                    if (32 * sub + tile_row(r, hi) >= left) s[sub][r] = -INFINITY;
         }
         // where all keys share one bias s stays the plain product, and scale and bias go into the exponent's one step
         float most = s[0][0];
@@ -129,24 +129,28 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
                 for (int r = 0; r < 16; ++r) o[i][r] *= factor;
         }
         const float base = top == -INFINITY ? 0.f : top;
-        const float by = a.scale * kLog2e, shift = (apart - base) * kLog2e;
+        if (BIAS && near) {
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+            for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f((s[r / 16][r % 16] - base) * kLog2e);
+        } else {
+            const float by = a.scale * kLog2e, shift = (apart - base) * kLog2e;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float x = near ? (s[sub][r] - base) * kLog2e : __builtin_fmaf(s[sub][r], by, shift);
-                s[sub][r] = __builtin_amdgcn_exp2f(x);
-                total += s[sub][r];
-            }
+            for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r / 16][r % 16], by, shift));
+        }
+#pragma unroll
+        for (int r = 0; r < 32; ++r) total += s[r / 16][r % 16];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
             const s16x8 p = rounded<E>(s[step / 2], step % 2);
 #pragma unroll
             for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(tile[now][1], 16 * step, i, lane), p, o[i]);
         }
+        feed<4 * kParts, 2, 4>();
+        __builtin_amdgcn_sched_barrier(0);
         if (more) {
-            ks.store(thread, tile[now ^ 1][0]);
-            vs.store(thread, tile[now ^ 1][1]);
+            ks.store(tile[now ^ 1][0]);
+            vs.store(tile[now ^ 1][1]);
         }
         __syncthreads();
         now ^= 1;
@@ -161,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
         for (int i = 0; i < kParts; ++i)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
-                const int at = 32 * i + row_of(4 * quad, hi);
+                const int at = 32 * i + mfma_row(4 * quad, hi);
                 if (at >= a.d) continue;
                 typename E::T y[4];
 #pragma unroll
@@ -178,7 +182,7 @@ __global__ __launch_bounds__(256, 2) void forward_kernel(AttendArgs a) {
         for (int i = 0; i < kParts; ++i)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
-                const int e = 32 * i + row_of(4 * quad, hi);
+                const int e = 32 * i + mfma_row(4 * quad, hi);
                 if (e >= a.d) continue;
                 *reinterpret_cast<f32x4*>(part + e) = f32x4{o[i][4 * quad], o[i][4 * quad + 1], o[i][4 * quad + 2], o[i][4 * quad + 3]};
             }
@@ -190,7 +194,7 @@ hipError_t launch_forward(const AttendArgs& a, hipStream_t stream) {
     const int64_t column_tiles = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns;
     const int64_t blocks = column_tiles * a.splits * (a.heads / a.pack) * a.batch;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const size_t lds = a.bias.table ? a.pack * (2 * a.bias.far + 7) * sizeof(float) : 0;
+    const size_t lds = a.bias.table ? a.pack * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     auto kernel = a.bias.table ? forward_kernel<E, DP, true> : forward_kernel<E, DP, false>;
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(a);
     return hipGetLastError();

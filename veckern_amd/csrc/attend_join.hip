@@ -5,39 +5,34 @@
 namespace vk {
 namespace attend {
 
-// One wave per query row: out = sum of exp(top_i - top) part_i / sum of exp(top_i - top) total_i. Two elements a lane.
+// out = sum of exp(top_i - top) part_i / sum of exp(top_i - top) total_i over the splits i; a thread takes four elements of a row.
 template <class E>
 __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
-    const int lane = threadIdx.x % 64, groups = a.heads / a.pack, columns = a.tokens * a.pack;
-    const int64_t rows = static_cast<int64_t>(a.batch) * groups * columns;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
-    if (row >= rows) return;
+    const int groups = a.heads / a.pack, columns = a.tokens * a.pack, quads = a.d / 4;
+    const int64_t rows = static_cast<int64_t>(a.batch) * groups * columns, at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (at >= rows * quads) return;
+    const int64_t row = at / quads;
+    const int e = static_cast<int>(at - row * quads) * 4;
     float top = -INFINITY;
-    for (int i = lane; i < a.splits; i += 64) top = fmaxf(top, a.stat[i * rows + row].x);
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.stat[i * rows + row].x);
     const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f, x = 0.f, y = 0.f;
+    float total = 0.f;
+    f32x4 x{};
     for (int i = 0; i < a.splits; ++i) {
         const float2 s = a.stat[i * rows + row];
         const float w = __builtin_amdgcn_exp2f((s.x - base) * kLog2e);
         total = __builtin_fmaf(w, s.y, total);
-        if (2 * lane < a.d) {
-            const float2 p = *reinterpret_cast<const float2*>(a.part + (i * rows + row) * a.d + 2 * lane);
-            x = __builtin_fmaf(w, p.x, x);
-            y = __builtin_fmaf(w, p.y, y);
-        }
+        x += w * *reinterpret_cast<const f32x4*>(a.part + (i * rows + row) * a.d + e);
     }
     const int c = row % columns, group = row / columns % groups, b = row / columns / groups;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const float factor = total == 0.f ? 0.f : 1.f / total;
-    if (2 * lane < a.d) {
-        typename E::T z[2] = {(typename E::T)(x * factor), (typename E::T)(y * factor)};
-        char* out = static_cast<char*>(a.out.p) + (b * a.out.outer + token * a.out.middle + head * a.out.head) * 2;
-        *reinterpret_cast<unsigned*>(out + 4 * lane) = *reinterpret_cast<unsigned*>(z);
-    }
-    if (a.lse && lane == 0)
-        a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
+    typename E::T z[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] = (typename E::T)(x[j] * factor);
+    char* out = static_cast<char*>(a.out.p) + (b * a.out.outer + token * a.out.middle + head * a.out.head + e) * 2;
+    *reinterpret_cast<u32x2*>(out) = *reinterpret_cast<u32x2*>(z);
+    if (a.lse && e == 0) a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
 }
 
 // One wave per (bucket, head).
@@ -56,9 +51,10 @@ __global__ __launch_bounds__(256) void table_kernel(AttendGradArgs g, int parts)
 }  // namespace attend
 
 hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stream) {
-    const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.tokens;
+    const int64_t blocks = (static_cast<int64_t>(a.batch) * a.heads * a.tokens * (a.d / 4) + 255) / 256;
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     auto kernel = type == kAttendBf16 ? attend::combine_kernel<attend::Bf16> : attend::combine_kernel<attend::F16>;
-    kernel<<<static_cast<unsigned>((rows + 3) / 4), 256, 0, stream>>>(a);
+    kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(a);
     return hipGetLastError();
 }
 

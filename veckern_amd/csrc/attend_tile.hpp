@@ -30,11 +30,17 @@ struct F16 {
     }
 };
 
-// In the 32x32 result of a matrix instruction a lane holds column lane % 32 and the rows row_of(r, lane / 32), r = 0..15.
-__device__ __forceinline__ constexpr int row_of(int r, int hi) { return 8 * (r / 4) + 4 * hi + r % 4; }
+// A 32x32 result of a matrix instruction: a lane holds column lane % 32 and the rows mfma_row(r, lane / 32), r = 0..15.
+__device__ __forceinline__ constexpr int mfma_row(int r, int hi) { return 8 * (r / 4) + 4 * hi + r % 4; }
+// Products over a tile's rows take them in an order of their own: row tile_row(r, hi) of the tile stands where the matrix
+// instruction has row mfma_row(r, hi). Four results that a lane holds next to each other are then four rows apart.
+__device__ __forceinline__ constexpr int tile_row(int r, int hi) { return 16 * (r / 8) + 4 * (r % 4) + 2 * (r / 4 % 2) + hi; }
+// The tile's row where the matrix instruction has row m, and back.
+__device__ __forceinline__ constexpr int row_at(int m) { return m / 16 * 16 + 4 * (m % 4) + 2 * (m / 8 % 2) + m / 4 % 2; }
+__device__ __forceinline__ constexpr int place_of(int row) { return row / 16 * 16 + row % 16 / 4 + 8 * (row / 2 % 2) + 4 * (row % 2); }
 
-// Eight of a lane's results, rounded, as the other operand of the next product. Its 16 contracted indices are then in the
-// order (hi, j) -> 8 * (j / 4) + 4 * hi + j % 4, which transposed() gives the first operand too, so no lane exchanges data.
+// Eight of a lane's results, rounded, as the other operand of the next product over the tile's rows. transposed() gives the
+// first operand the same order of rows, so no lane exchanges data.
 template <class E>
 __device__ __forceinline__ s16x8 rounded(const f32x16& x, int half) {
     typename E::x8 y;
@@ -52,73 +58,81 @@ __device__ __forceinline__ float both_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// Tiles in LDS: rows of DP 16-bit elements, in 16-byte chunks; chunk c of a row lies at place c ^ spread(row). A
-// ds_read_b128 of 16 consecutive lanes takes one chunk of 16 rows, and the transposing read of 32 lanes four chunks of four
-// consecutive rows: with this order either covers the 64 banks of 4 bytes once.
+// Tiles in LDS: rows of DP 16-bit elements, 16 bytes apart. A ds_read_b128 of 16 consecutive lanes takes 16 bytes of 16 rows,
+// the transposing read of 32 lanes 64 bytes of rows that are four apart: either covers the 64 banks of 4 bytes once. Every
+// place of a tile is one lane's address plus a constant, so the reads take two address registers in all.
 template <int DP>
-__device__ __forceinline__ constexpr int spread(int row) {
-    return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-}
+constexpr int kPitch = DP * 2 + 16;
+template <int DP, int ROWS>
+constexpr int kTileBytes = ROWS * kPitch<DP>;
 
 // Copies ROWS rows of a tensor into such a tile through registers; rows past `valid` and elements past d become zero (the
 // buffer descriptor's range check), so nothing of what lies there, infinities and NaN included, reaches a product.
 template <int DP, int ROWS, int THREADS>
 struct Copier {
-    static constexpr int kChunks = DP / 8, kEach = ROWS * kChunks / THREADS;
-    static_assert(ROWS * kChunks % THREADS == 0, "every thread copies the same number of chunks");
+    static constexpr int kChunks = DP / 8, kEach = ROWS * kChunks / THREADS, kRows = THREADS / kChunks;
+    static_assert(ROWS * kChunks % THREADS == 0 && THREADS % kChunks == 0, "every thread copies the same chunk of some rows");
     static constexpr int kOut = int(0x80000000u);  // past every descriptor's range
-    int offset[kEach];
+    int row, offset, step, to;
     u32x4 held[kEach];
 
     __device__ void init(int thread, int64_t stride, int d) {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int p = thread + THREADS * i, row = p / kChunks, chunk = (p % kChunks) ^ spread<DP>(row);
-            offset[i] = chunk * 8 < d ? static_cast<int>(row * stride * 2) + chunk * 16 : kOut;
-        }
+        row = thread / kChunks;
+        const int chunk = thread % kChunks;
+        offset = chunk * 8 < d ? static_cast<int>(row * stride * 2) + chunk * 16 : kOut;
+        step = static_cast<int>(kRows * stride * 2);
+        to = row * kPitch<DP> + chunk * 16;
     }
-    __device__ void load(int thread, const void* base, int valid) {
+    __device__ void load(const void* base, int valid) {
         auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int row = (thread + THREADS * i) / kChunks;
-            held[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row < valid ? offset[i] : kOut, 0, 0);
-        }
+        for (int i = 0; i < kEach; ++i)
+            held[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row + kRows * i < valid ? offset + step * i : kOut, 0, 0);
     }
-    __device__ void store(int thread, void* tile) const {
+    __device__ void store(char* tile) const {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) static_cast<u32x4*>(tile)[thread + THREADS * i] = held[i];
+        for (int i = 0; i < kEach; ++i) *reinterpret_cast<u32x4*>(tile + to + kRows * i * kPitch<DP>) = held[i];
     }
 };
 
-// First operand, rows as they lie: lane row = base + lane % 32, contracted elements 16 * step + 8 * hi ...
+// First operand, rows as they lie: 32 rows from `base` on, contracted elements 16 * step + 8 * hi ...
 template <int DP>
-__device__ __forceinline__ s16x8 straight(const void* tile, int base, int step, int lane) {
-    const int row = base + lane % 32;
-    return static_cast<const s16x8*>(tile)[row * (DP / 8) + ((2 * step + lane / 32) ^ spread<DP>(row))];
+__device__ __forceinline__ s16x8 straight(const char* tile, int base, int step, int lane) {
+    return *reinterpret_cast<const s16x8*>(tile + row_at(lane % 32) * kPitch<DP> + lane / 32 * 16 + base * kPitch<DP> + step * 32);
 }
-// First operand, transposed: lane row = element 32 * part + lane % 32, contracted over the tile's rows base + (hi, j).
+// First operand, transposed: lane row = element 32 * part + lane % 32, contracted over the 16 rows from `base` on.
 template <int DP>
-__device__ __forceinline__ s16x8 transposed(const void* tile, int base, int part, int lane) {
+__device__ __forceinline__ s16x8 transposed(const char* tile, int base, int part, int lane) {
     typedef __attribute__((address_space(3))) s16x4 L;
+    const char* at = tile + (4 * (lane % 16 / 4) + lane / 32) * kPitch<DP> + lane % 32 / 16 * 32 + lane % 4 * 8;
     s16x8 y;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        const int row = base + 8 * half + 4 * (lane / 32) + lane % 16 / 4;
-        const int chunk = 4 * part + lane % 32 / 16 * 2 + lane % 4 / 2;
-        const char* at = static_cast<const char*>(tile) + (row * (DP / 8) + (chunk ^ spread<DP>(row))) * 16 + lane % 2 * 8;
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)at);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L*)(at + (base + 2 * half) * kPitch<DP> + part * 64));
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[4 * half + j] = x[j];
     }
     return y;
 }
-// Second operand from global memory: column lane % 32 is the row at `p` (nullptr: zeros), elements 16 * step + 8 * hi ...
-__device__ __forceinline__ s16x8 column(const void* p, int step, int hi, int d) {
+// Second operand from global memory: column lane % 32 is the row `offset` elements into the tensor (used = false: zeros),
+// elements 16 * step + 8 * hi ... What is not there is read at the tensor's start instead, so that no load waits for a branch.
+__device__ __forceinline__ s16x8 column(const AttendView& v, int64_t offset, bool used, int step, int hi, int d) {
     const int at = 16 * step + 8 * hi;
-    s16x8 zero = {};
-    return p && at < d ? *reinterpret_cast<const s16x8*>(static_cast<const char*>(p) + at * 2) : zero;
+    const bool there = used && at < d;
+    const s16x8 x = *reinterpret_cast<const s16x8*>(static_cast<const char*>(v.p) + (there ? (offset + at) * 2 : 0));
+    const s16x8 zero = {};
+    return there ? x : zero;
 }
+
+// What lanes of a wave wrote to LDS before is there for its other lanes after.
+__device__ __forceinline__ void between_lanes() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// How much a running maximum may be below the true one (attend_forward.inl).
+constexpr float kSlack = 5.f;
 
 // log(total) + top in two parts, so that nothing of log(total) is lost where every key of a row has a bias of the type's
 // lowest value.
@@ -185,11 +199,11 @@ __device__ __forceinline__ int xcd_place(int id, int total) {
     return x * q + min(x, extra) + i;
 }
 
-// The bias by distance in LDS: held[i] = table[bucket(i - far - 3)][head], i in [0, 2 * far + 7). Every distance
-// from `far` on shares the last bucket of its side, so an index may be clamped; the three more at either end let four
-// neighbouring distances be clamped as one.
-__device__ __forceinline__ int bias_places(int far) { return 2 * far + 7; }
-__device__ __forceinline__ int bias_index(int far, int x) { return min(max(x + far + 3, 0), 2 * far + 3); }
+// The bias by distance in LDS: held[i] = table[bucket(i - far - kPad)][head], i in [0, 2 * far + 2 * kPad]. Every distance from
+// `far` on shares the last bucket of its side, so an index may be clamped; the pad at either end lets 16 neighbouring distances
+// be clamped as one.
+__device__ __forceinline__ int bias_places(int far) { return 2 * far + 2 * kPad + 1; }
+__device__ __forceinline__ int bias_index(int far, int x) { return min(max(x + far + kPad, 0), 2 * far + kPad); }
 __device__ __forceinline__ int bucket_of(const AttendBias& s, int x) {
     const int a = s.two_sided ? abs(x) : max(-x, 0), exact = s.side / 2;
     int bucket = a;
@@ -208,7 +222,7 @@ template <class E>
 __device__ __forceinline__ void fill_bias(const AttendBias& s, int head, float* held, int thread, int threads) {
     for (int i = thread; i < bias_places(s.far); i += threads) {
         const auto* t = static_cast<const typename E::T*>(s.table);
-        held[i] = static_cast<float>(t[bucket_of(s, i - s.far - 3) * s.bucket_stride + head * s.head_stride]);
+        held[i] = static_cast<float>(t[bucket_of(s, i - s.far - kPad) * s.bucket_stride + head * s.head_stride]);
     }
 }
 // Whether all distances in [least, most] share one bucket of the far ends (one-sided: all that are not negative do too).
@@ -221,17 +235,34 @@ __device__ __forceinline__ bool far_apart(const AttendBias& s, int least, int mo
 constexpr float kLargeBias = 1e4f;
 
 // The logits of a 32 x 32 tile, scores * scale + bias, in natural units (a type's lowest value, as a bias that almost never
-// lets a key through, would overflow in log2 units). x0: the distance at the lane's row_of(0), step: the
-// distance's change from row to row.
+// lets a key through, would overflow in log2 units). x0: the distance at tile_row(0, hi) of the lane; STEP: how it changes
+// from row to row.
 template <int STEP>
 __device__ __forceinline__ void add_bias(f32x16& s, float scale, const float* held, int far, int x0) {
 #pragma unroll
-    for (int quad = 0; quad < 4; ++quad) {
-        const int x = x0 + STEP * 8 * quad;
-        const float* at = held + bias_index(far, STEP > 0 ? x : x - 3);
+    for (int part = 0; part < 2; ++part) {
+        const int x = x0 + STEP * 16 * part;
+        const float* at = held + bias_index(far, STEP > 0 ? x : x - 14);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * quad + j] = __builtin_fmaf(s[4 * quad + j], scale, at[STEP > 0 ? j : 3 - j]);
+        for (int r = 0; r < 8; ++r)
+            s[8 * part + r] = __builtin_fmaf(s[8 * part + r], scale, at[STEP > 0 ? tile_row(r, 0) : 14 - tile_row(r, 0)]);
     }
 }
+
+// Instruction order of a run of `n` products of the matrix cores whose first operands come from LDS, `reads` reads each: the
+// reads are kept `ahead` products in front, as a read takes about as long as three to four products, and `others` vector
+// instructions of another part of the tile, that runs beside it, follow each product.
+template <int n, int reads, int ahead, int others = 0>
+__device__ __forceinline__ void feed() {
+    __builtin_amdgcn_sched_group_barrier(0x100, reads * ahead, 0);
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i < n - ahead) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+        if (others) __builtin_amdgcn_sched_group_barrier(0x002, others, 0);
+    }
+}
+// Where one run ends and the next begins.
+__device__ __forceinline__ void between_runs() { __builtin_amdgcn_sched_barrier(0); }
 
 }  // namespace vk::attend
