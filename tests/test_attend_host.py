@@ -45,7 +45,7 @@ def test_missing_tensors_and_workspaces_are_refused():
     assert lib.vk_attend(None, None, 0, None) == invalid
     assert lib.vk_attend_workspace(ctypes.byref(arguments()), None) == invalid
     assert lib.vk_bias_bucket(1, 32, 128, 1, None) == invalid
-    a = arguments()
+    a = arguments(tokens=40)  # few blocks and several tiles of keys: their parts are joined in a workspace
     assert lib.vk_attend(ctypes.byref(a), None, 0, None) == invalid and b"q is NULL" in lib.vk_last_error()
     # host addresses that are never read: the call is refused before a launch
     held = (ctypes.c_char * 4096)()

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
@@ -71,15 +72,15 @@ def _view(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> _Tens
     return _Tensor(t.data_ptr(), (a, b, c))
 
 
-def _indices(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, strided: bool) -> int:
+def _indices(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor, strided: bool) -> None:
     if t.shape != shape or t.dtype != torch.int32 or t.device != like.device:
         _refuse(f"{name} must be {list(shape)} int32 on {like.device}, not {list(t.shape)} {t.dtype} on {t.device}")
     if not strided and not t.is_contiguous():
         _refuse(f"{name} must be contiguous")
-    return t.data_ptr()
 
 
-def _arguments(q, keys, values, out, rows, lengths, bias, q_start, scale) -> _Attention:
+def _arguments(q, keys, values, rows, lengths, bias, q_start, scale) -> _Attention:
+    """Everything of a call but its addresses."""
     if not q.is_cuda:
         _refuse("queries must be on a GPU")
     if q.dim() != 4 or keys.dim() != 4:
@@ -105,52 +106,108 @@ def _arguments(q, keys, values, out, rows, lengths, bias, q_start, scale) -> _At
         if rows.dim() != 2:
             _refuse("rows must be [batch, passages]")
         a.passages = rows.shape[1]
-        a.rows = _indices(rows, "rows", (batch, rows.shape[1]), q, True) or q.data_ptr()  # without elements: any address
+        _indices(rows, "rows", (batch, rows.shape[1]), q, True)
+        a.rows = 1  # there are some; the address follows
         a.rows_stride = rows.stride()
     a.scale = 1.0 / math.sqrt(d) if scale is None else scale
     a.q = _view(q, "queries", q.shape, q)
     a.k = _view(keys, "keys", keys.shape, q)
     a.v = _view(values, "values", keys.shape, q)
-    a.out = _view(out, "out", q.shape, q)
     if lengths is not None:
-        a.lengths = _indices(lengths, "lengths", (bank,), q, False)
+        _indices(lengths, "lengths", (bank,), q, False)
     if bias is not None:
         t = bias.table
         if t.dim() != 2 or t.shape[0] == 0 or t.shape[1] != heads or t.dtype != q.dtype or t.device != q.device:
             _refuse(f"the bias table must be [buckets, {heads}] {q.dtype} on {q.device}, not {list(t.shape)} {t.dtype} on "
                     f"{t.device}")
-        a.table, a.table_stride, a.buckets = t.data_ptr(), t.stride(), t.shape[0]
+        a.table, a.table_stride, a.buckets = 1, t.stride(), t.shape[0]
         a.max_distance, a.two_sided = bias.max_distance, bias.two_sided
     if isinstance(q_start, torch.Tensor):
-        a.q_starts = _indices(q_start, "q_start", (batch,), q, False)
+        _indices(q_start, "q_start", (batch,), q, False)
     else:
         a.q_start = q_start
     return a
 
 
-def _launch(call, measure, arguments, device):
+class _Plan(NamedTuple):
+    """What calls with the same sizes, strides, types and devices share: the arguments but for the addresses."""
+
+    image: bytes
+    forward_bytes: int
+    backward_bytes: int
+    lse_shape: tuple
+
+
+_plans: dict = {}
+_MOST_PLANS = 512
+
+
+def _kind(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _plan(q, keys, values, rows, lengths, bias, q_start, scale) -> _Plan:
+    key = (_kind(q), _kind(keys), _kind(values), _kind(rows), _kind(lengths),
+           None if bias is None else (_kind(bias.table), bias.max_distance, bias.two_sided),
+           _kind(q_start) if isinstance(q_start, torch.Tensor) else q_start, scale)
+    plan = _plans.get(key)
+    if plan is None:
+        a = _arguments(q, keys, values, rows, lengths, bias, q_start, scale)
+        lib, forward, backward = library(), ctypes.c_size_t(), ctypes.c_size_t()
+        _check(lib.vk_attend_workspace(ctypes.byref(a), ctypes.byref(forward)))
+        _check(lib.vk_attend_backward_workspace(ctypes.byref(a), ctypes.byref(backward)))
+        plan = _Plan(bytes(a), forward.value, backward.value, (a.batch, a.heads, a.tokens, 2))
+        if len(_plans) >= _MOST_PLANS:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
+
+
+_ADDRESS = struct.Struct("P")
+_AT = {name: getattr(_Attention, name).offset for name in ("q", "k", "v", "out", "rows", "lengths", "lse", "table", "q_starts")}
+_OUT_STRIDE = _AT["out"] + _Tensor.stride.offset
+_STRIDES = struct.Struct("3q")
+
+
+def _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start) -> _Attention:
+    a, put = bytearray(plan.image), _ADDRESS.pack_into
+    put(a, _AT["q"], q.data_ptr())
+    put(a, _AT["k"], keys.data_ptr())
+    put(a, _AT["v"], values.data_ptr())
+    put(a, _AT["out"], out.data_ptr())
+    _STRIDES.pack_into(a, _OUT_STRIDE, *out.stride()[:3])
+    if rows is not None:
+        put(a, _AT["rows"], rows.data_ptr() or 1)  # without elements: any address, there is nothing to read
+    if lengths is not None:
+        put(a, _AT["lengths"], lengths.data_ptr())
+    if lse is not None:
+        put(a, _AT["lse"], lse.data_ptr())
+    if bias is not None:
+        put(a, _AT["table"], bias.table.data_ptr())
+    if isinstance(q_start, torch.Tensor):
+        put(a, _AT["q_starts"], q_start.data_ptr())
+    return _Attention.from_buffer(a)
+
+
+def _launch(call, size, device):
     """Runs ``call(workspace, bytes, stream)`` on the device's current stream."""
-    size = ctypes.c_size_t()
-    _check(measure(arguments, ctypes.byref(size)))
-    work = torch.empty(size.value, dtype=torch.uint8, device=device) if size.value else None
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    at = work.data_ptr() if size else None
     stream = torch.cuda.current_stream(device).cuda_stream
-    at = work.data_ptr() if work is not None else None
     if device.index == torch.cuda.current_device():
-        _check(call(at, size.value, stream))
+        _check(call(at, size, stream))
     else:
         with torch.cuda.device(device):
-            _check(call(at, size.value, stream))
+            _check(call(at, size, stream))
 
 
 def _forward(q, keys, values, rows, lengths, bias, q_start, scale, with_lse):
+    plan = _plan(q, keys, values, rows, lengths, bias, q_start, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a = _arguments(q, keys, values, out, rows, lengths, bias, q_start, scale)
-    lse = None
-    if with_lse:
-        lse = torch.empty((a.batch, a.heads, a.tokens, 2), dtype=torch.float32, device=q.device)
-        a.lse = lse.data_ptr()
-    lib, r = library(), ctypes.byref(a)
-    _launch(lambda at, size, stream: lib.vk_attend(r, at, size, stream), lib.vk_attend_workspace, r, q.device)
+    lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device) if with_lse else None
+    a = _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start)
+    vk_attend = library().vk_attend
+    _launch(lambda at, size, stream: vk_attend(a, at, size, stream), plan.forward_bytes, q.device)
     return out, lse
 
 
@@ -207,25 +264,28 @@ def attend_backward(d_out: torch.Tensor, q: torch.Tensor, keys: torch.Tensor, va
                     bias: Optional[RelativeBias] = None, q_start=0, scale: Optional[float] = None) -> Gradients:
     """The gradients of a loss whose gradient by ``out`` is ``d_out``; ``out`` and ``lse`` as ``attend`` returned them for
     the same arguments. With ``rows`` the bank is a constant and has none."""
-    a = _arguments(q, keys, values, out, rows, lengths, bias, q_start, scale)
-    if lse.shape != (a.batch, a.heads, a.tokens, 2) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
-        _refuse(f"lse must be contiguous [{a.batch}, {a.heads}, {a.tokens}, 2] float32 on {q.device}")
-    a.lse = lse.data_ptr()
+    plan = _plan(q, keys, values, rows, lengths, bias, q_start, scale)
+    if lse.shape != plan.lse_shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        _refuse(f"lse must be contiguous {list(plan.lse_shape)} float32 on {q.device}")
+    _view(out, "out", q.shape, q)
+    a = _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start)
     g = _AttentionGrad()
     g.d_out = _view(d_out, "d_out", q.shape, q)
 
     def like(t):
         return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
+    def whole(t):
+        return _Tensor(t.data_ptr(), t.stride()[:3])
+
     d_q, d_k, d_v, d_table = like(q), None, None, None
-    g.d_q = _view(d_q, "d_q", q.shape, q)
+    g.d_q = whole(d_q)
     if rows is None:
         d_k, d_v = like(keys), like(values)
-        g.d_k, g.d_v = _view(d_k, "d_k", keys.shape, q), _view(d_v, "d_v", keys.shape, q)
+        g.d_k, g.d_v = whole(d_k), whole(d_v)
     if bias is not None:
         d_table = like(bias.table)
         g.d_table = d_table.data_ptr()
-    lib, r, s = library(), ctypes.byref(a), ctypes.byref(g)
-    _launch(lambda at, size, stream: lib.vk_attend_backward(r, s, at, size, stream), lib.vk_attend_backward_workspace, r,
-            q.device)
+    vk_attend_backward = library().vk_attend_backward
+    _launch(lambda at, size, stream: vk_attend_backward(a, g, at, size, stream), plan.backward_bytes, q.device)
     return Gradients(d_q, d_k, d_v, d_table)

@@ -11,6 +11,7 @@ namespace vk {
 constexpr int kMostEdges = 128;      // bucket edges of a one-sided bias of 256 buckets
 constexpr int kMostDistance = 1024;  // largest max_distance: the bias by distance, and its gradient, are held in LDS
 constexpr int kPad = 15;             // places at either end of the bias by distance (attend_tile.hpp)
+constexpr int kMostBiasBytes = 16384;  // biases by distance of the heads that share a block's columns; else a head alone
 constexpr int kKeyTile = 64;         // keys that a block of the tile kernels holds at once
 constexpr int kFewPassages = 512;    // passages that a block of the few-columns kernel holds the rows of
 constexpr int kColumns = 128;        // query columns of a block of the tile kernels

@@ -132,7 +132,19 @@ AttendArgs args_of(const vk_attention* x, bool tensors) {
     a.lse = reinterpret_cast<float2*>(x->lse);
     valid(reinterpret_cast<uintptr_t>(x->lse) % 8 == 0, "lse is not 8-byte aligned");
     if (x->table) {
-        a.bias = bias_of(x->buckets, x->max_distance, x->two_sided != 0);
+        // its powers take microseconds: the thread's last layout is kept, by its three numbers
+        static thread_local struct {
+            size_t buckets = 0, max_distance = 0;
+            bool two_sided = false;
+            AttendBias bias;
+        } last;
+        if (last.buckets != x->buckets || last.max_distance != x->max_distance || last.two_sided != (x->two_sided != 0)) {
+            last.bias = bias_of(x->buckets, x->max_distance, x->two_sided != 0);
+            last.buckets = x->buckets;
+            last.max_distance = x->max_distance;
+            last.two_sided = x->two_sided != 0;
+        }
+        a.bias = last.bias;
         a.bias.table = x->table;
         a.bias.bucket_stride = x->table_stride[0];
         a.bias.head_stride = x->table_stride[1];
@@ -166,7 +178,7 @@ void split_keys(AttendArgs& a, int tile, int64_t blocks, int64_t wanted, int lea
 void plan_forward(AttendArgs& a) {
     const int share = a.heads / a.kv_heads;
     a.pack = share;
-    if (a.bias.table && static_cast<size_t>(share) * (2 * a.bias.far + 2 * vk::kPad + 1) * sizeof(float) > 16384) a.pack = 1;
+    if (a.bias.table && static_cast<size_t>(share) * (2 * a.bias.far + 2 * vk::kPad + 1) * sizeof(float) > vk::kMostBiasBytes) a.pack = 1;
     const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
     if (few_columns(a)) {
         const int per_row = (a.length + 31) / 32;  // a run of tiles touches one passage more than it fills

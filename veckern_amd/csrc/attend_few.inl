@@ -3,6 +3,8 @@
 // own columns' maxima, sums and outputs, which are joined in LDS at the end, so most calls are one launch and few blocks keep
 // many loads in flight: a wave has its next tile's K and V (16 KB at 128 elements a head) under way while it works on one. Nothing
 // waits at a barrier in between. Products, roundings and the raised maximum are those of the tile kernel (attend_forward.inl).
+#include <atomic>
+
 #include "attend_tile.hpp"
 
 namespace vk::attend {
@@ -196,9 +198,19 @@ hipError_t launch_few(const AttendArgs& a, hipStream_t stream) {
     const size_t lds = kFewTiles<DP> + kFewPassages * sizeof(int2) +
                        (a.bias.table ? a.pack * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0);
     auto kernel = a.bias.table ? few_kernel<E, DP, true> : few_kernel<E, DP, false>;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(lds));
+    // more LDS than a kernel may have unasked; asked for once a device, for any bias
+    static std::atomic<uint64_t> asked[2];
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return e;
+    std::atomic<uint64_t>& done = asked[a.bias.table != nullptr];
+    const uint64_t bit = uint64_t(1) << (device % 64);
+    if (device >= 64 || !(done.load(std::memory_order_relaxed) & bit)) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                kFewTiles<DP> + static_cast<int>(kFewPassages * sizeof(int2)) + kMostBiasBytes);
+        if (e != hipSuccess) return e;
+        done.fetch_or(bit, std::memory_order_relaxed);
+    }
     kernel<<<static_cast<unsigned>(blocks), 64 * kFewWaves, lds, stream>>>(a);
     return hipGetLastError();
 }

@@ -14,10 +14,12 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
     const int64_t row = at / quads;
     const int e = static_cast<int>(at - row * quads) * 4;
     float top = -INFINITY;
+#pragma unroll 4
     for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.stat[i * rows + row].x);
     const float base = top == -INFINITY ? 0.f : top;
     float total = 0.f;
     f32x4 x{};
+#pragma unroll 4
     for (int i = 0; i < a.splits; ++i) {
         const float2 s = a.stat[i * rows + row];
         const float w = __builtin_amdgcn_exp2f((s.x - base) * kLog2e);
@@ -42,6 +44,7 @@ __global__ __launch_bounds__(256) void table_kernel(AttendGradArgs g, int parts)
     if (at >= g.a.heads * g.a.bias.buckets) return;
     const int head = at % g.a.heads, bucket = at / g.a.heads;
     float x = 0.f;
+#pragma unroll 4
     for (int i = lane; i < parts; i += 64) x += g.table_part[(static_cast<int64_t>(i) * g.a.heads + head) * g.a.bias.buckets + bucket];
 #pragma unroll
     for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
