@@ -131,19 +131,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_q_kernel(AttendGra
     }
     __syncthreads();
     const char *k, *v;
-    auto products = [&](f32x16& s, f32x16& dp, int sub) {
-        s = dp = f32x16{};
+    auto products = [&](f32x16 (&s)[2], f32x16 (&dp)[2]) {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s);
+        for (int sub = 0; sub < 2; ++sub) {
+            s[sub] = dp[sub] = f32x16{};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) dp = E::mfma(straight<DP>(v, 32 * sub, i, lane), df[i], dp);
+            for (int i = 0; i < kSteps; ++i) {
+                s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
+                dp[sub] = E::mfma(straight<DP>(v, 32 * sub, i, lane), df[i], dp[sub]);
+            }
+        }
     };
-    auto gather = [&](const f32x16& ds, int sub) {
+    auto gather = [&](const f32x16 (&ds)[2]) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const s16x8 x = rounded<E>(ds, half);
+        for (int half = 0; half < 4; ++half) {
+            const s16x8 x = rounded<E>(ds[half / 2], half % 2);
 #pragma unroll
-            for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 32 * sub + 16 * half, i, lane), x, dq[i]);
+            for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 16 * half, i, lane), x, dq[i]);
         }
     };
     while (more) {
@@ -153,65 +157,54 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_q_kernel(AttendGra
         if (more) load();
         k = tile[now][0];
         v = tile[now][1];
-        bool plain = left >= kKeyTile;  // all keys are there, and share one bias
+        bool near = false;  // the tile's keys do not share one bias
         float apart = 0.f;
         int t0 = 0;
         if constexpr (BIAS) {
             t0 = __builtin_amdgcn_readfirstlane(position);
             apart = held[bias_index(a.bias.far, first - position)];
-            plain = plain && far_apart(a.bias, first - (t0 + 31), first + kKeyTile - 1 - t0) && !__any(fabsf(apart) > kLargeBias);
+            near = !far_apart(a.bias, first - (t0 + 31), first + kKeyTile - 1 - t0) || __any(fabsf(apart) > kLargeBias);
         }
         f32x16 s[2], dp[2];
-        if (plain) {
-            const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
-            auto weights = [&](f32x16& s, const f32x16& dp) {
+        between_runs();
+        products(s, dp);
+        feed<4 * kSteps, 1, 4>();
+        between_runs();
+        if (BIAS && near) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], scale_log2, shift)) * (dp[r] - delta);
-            };
-            // the two halves of the tile one step apart: the weights of one are taken beside the products of the other
-            between_runs();
-            products(s[0], dp[0], 0);
-            feed<2 * kSteps, 1, 4>();
-            between_runs();
-            products(s[1], dp[1], 1);
-            weights(s[0], dp[0]);
-            feed<2 * kSteps, 1, 4, 64 / kSteps>();
-            between_runs();
-            gather(s[0], 0);
-            weights(s[1], dp[1]);
-            feed<2 * kParts, 2, 2, 128 / kSteps>();
-            between_runs();
-            gather(s[1], 1);
-            feed<2 * kParts, 2, 3>();
-            between_runs();
-            if constexpr (BIAS) {
+            for (int sub = 0; sub < 2; ++sub) {
+                add_bias<1>(s[sub], a.scale, held, a.bias.far, first + 32 * sub + hi - position);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[sub][r] = __builtin_fmaf(s[sub][r] - lse.x, kLog2e, lse.y);
+            }
+        } else {
+            const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
+#pragma unroll
+            for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = __builtin_fmaf(s[r / 16][r % 16], scale_log2, shift);
+        }
+#pragma unroll
+        for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
+        if (left < kKeyTile) {
+#pragma unroll
+            for (int r = 0; r < 32; ++r)
+                if (r / 16 * 32 + tile_row(r % 16, hi) >= left) s[r / 16][r % 16] = 0.f;
+        }
+        if constexpr (BIAS) {
+            if (near) {
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) add_by_distance(s[sub], skew, sums, a.bias.far, first + 32 * sub - t0, lane, below, above);
+            } else {
                 float all = 0.f;
 #pragma unroll
                 for (int r = 0; r < 32; ++r) all += s[r / 16][r % 16];
                 if (first < position) below += all;
                 else above += all;
             }
-        } else {
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                products(s[sub], dp[sub], sub);
-                f32x16& x = s[sub];
-                if constexpr (BIAS) {
-                    add_bias<1>(x, a.scale, held, a.bias.far, first + 32 * sub + hi - position);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) x[r] *= a.scale;
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - lse.x, kLog2e, lse.y));
-                    x[r] = 32 * sub + tile_row(r, hi) < left ? p * (dp[sub][r] - delta) : 0.f;
-                }
-                if constexpr (BIAS) add_by_distance(x, skew, sums, a.bias.far, first + 32 * sub - t0, lane, below, above);
-                gather(x, sub);
-            }
         }
+        between_runs();
+        gather(s);
+        feed<4 * kParts, 2, 3>();
+        between_runs();
         if (more) {
             ks.store(tile[now ^ 1][0]);
             vs.store(tile[now ^ 1][1]);
@@ -312,8 +305,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_kv_kernel(AttendGr
             ds.load(static_cast<const char*>(g.d_out.p) + (b * g.d_out.outer + first * g.d_out.middle + head * g.d_out.head) * 2, valid);
             if (thread < kQueries) {
                 const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + first + thread;
+                // nothing is computed from them before store(): that would wait for all loads under way
                 lse = thread < valid ? a.lse[at] : make_float2(-INFINITY, 0.f);
-                lse = make_float2(lse.x == -INFINITY ? INFINITY : lse.x, lse.y * -kLog2e);
                 delta = thread < valid ? g.delta[at] : 0.f;
             }
         };
@@ -322,9 +315,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_kv_kernel(AttendGr
             ds.store(tile[to][1]);
             if (thread < kQueries) {
                 const int at = place_of(thread);
-                stat[to][0][at] = lse.x;
-                stat[to][1][at] = lse.y;
-                stat[to][2][at] = __builtin_fmaf(lse.x, -kLog2e, lse.y);
+                const float value = lse.x == -INFINITY ? INFINITY : lse.x, low = lse.y * -kLog2e;
+                stat[to][0][at] = value;
+                stat[to][1][at] = low;
+                stat[to][2][at] = __builtin_fmaf(value, -kLog2e, low);
                 stat[to][3][at] = delta;
             }
         };
@@ -338,29 +332,26 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_kv_kernel(AttendGr
         auto of = [&](int which, int sub, int quad) {
             return *reinterpret_cast<const f32x4*>(&stat[now][which][32 * sub + mfma_row(4 * quad, hi)]);
         };
-        auto products = [&](f32x16& s, f32x16& dp, int sub) {
-            s = dp = f32x16{};
+        auto products = [&](f32x16 (&s)[2], f32x16 (&dp)[2]) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(q, 32 * sub, i, lane), kf[i], s);
+            for (int sub = 0; sub < 2; ++sub) {
+                s[sub] = dp[sub] = f32x16{};
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) dp = E::mfma(straight<DP>(d, 32 * sub, i, lane), vf[i], dp);
-        };
-        auto times_rest = [&](const f32x16& p, f32x16& dp, int sub) {
-#pragma unroll
-            for (int quad = 0; quad < 4; ++quad) {
-                const f32x4 e = of(3, sub, quad);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) dp[4 * quad + j] = p[4 * quad + j] * (dp[4 * quad + j] - e[j]);
+                for (int i = 0; i < kSteps; ++i) {
+                    s[sub] = E::mfma(straight<DP>(q, 32 * sub, i, lane), kf[i], s[sub]);
+                    dp[sub] = E::mfma(straight<DP>(d, 32 * sub, i, lane), vf[i], dp[sub]);
+                }
             }
         };
-        auto gather = [&](const f32x16& p, const f32x16& ds, int sub) {
+        auto gather = [&](const f32x16 (&p)[2], const f32x16 (&ds)[2]) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const s16x8 x = rounded<E>(p, half), y = rounded<E>(ds, half);
+            for (int half = 0; half < 4; ++half) {
+                const s16x8 x = rounded<E>(p[half / 2], half % 2), y = rounded<E>(ds[half / 2], half % 2);
 #pragma unroll
-                for (int i = 0; i < kParts; ++i) dv[i] = E::mfma(transposed<DP>(d, 32 * sub + 16 * half, i, lane), x, dv[i]);
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) dk[i] = E::mfma(transposed<DP>(q, 32 * sub + 16 * half, i, lane), y, dk[i]);
+                for (int i = 0; i < kParts; ++i) {
+                    dv[i] = E::mfma(transposed<DP>(d, 16 * half, i, lane), x, dv[i]);
+                    dk[i] = E::mfma(transposed<DP>(q, 16 * half, i, lane), y, dk[i]);
+                }
             }
         };
         while (more) {
@@ -376,61 +367,57 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void grad_kv_kernel(AttendGr
             if (more) load();
             q = tile[now][0];
             d = tile[now][1];
-            bool plain = true;  // all places share one bias
+            bool near = false;  // the tile's places do not share one bias
             float apart = 0.f;
             if constexpr (BIAS) {
                 const int k0 = key_tile * kColumns + wave * 32;
                 apart = bias_held[bias_index(a.bias.far, key - (from + start))];
-                plain = far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start)) &&
-                        !__any(fabsf(apart) > kLargeBias);
+                near = !far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start)) ||
+                       __any(fabsf(apart) > kLargeBias);
             }
             f32x16 s[2], dp[2];
-            if (plain) {
-                const float apart_log2 = apart * kLog2e;
-                auto weights = [&](f32x16& s, f32x16& dp, int sub) {
-#pragma unroll
-                    for (int quad = 0; quad < 4; ++quad) {
-                        const f32x4 one = of(2, sub, quad);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            s[4 * quad + j] = __builtin_amdgcn_exp2f(
-                                __builtin_fmaf(s[4 * quad + j], scale_log2, BIAS ? apart_log2 + one[j] : one[j]));
-                    }
-                    times_rest(s, dp, sub);
-                };
-                // the two halves of the tile one step apart: the weights of one are taken beside the products of the other
-                between_runs();
-                products(s[0], dp[0], 0);
-                feed<2 * kSteps, 1, 4>();
-                between_runs();
-                products(s[1], dp[1], 1);
-                weights(s[0], dp[0], 0);
-                feed<2 * kSteps, 1, 4, 64 / kSteps>();
-                between_runs();
-                gather(s[0], dp[0], 0);
-                weights(s[1], dp[1], 1);
-                feed<4 * kParts, 2, 2, 64 / kSteps>();
-                between_runs();
-                gather(s[1], dp[1], 1);
-                feed<4 * kParts, 2, 3>();
-                between_runs();
-            } else {
+            between_runs();
+            products(s, dp);
+            feed<4 * kSteps, 1, 4>();
+            between_runs();
+            if (BIAS && near) {
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub) {
-                    products(s[sub], dp[sub], sub);
-                    f32x16& x = s[sub];
-                    add_bias<-1>(x, a.scale, bias_held, a.bias.far, key - (from + start + 32 * sub + hi));
+                    add_bias<-1>(s[sub], a.scale, bias_held, a.bias.far, key - (from + start + 32 * sub + hi));
 #pragma unroll
                     for (int quad = 0; quad < 4; ++quad) {
                         const f32x4 l = of(0, sub, quad), low = of(1, sub, quad);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            x[4 * quad + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[4 * quad + j] - l[j], kLog2e, low[j]));
+                            s[sub][4 * quad + j] = __builtin_fmaf(s[sub][4 * quad + j] - l[j], kLog2e, low[j]);
                     }
-                    times_rest(x, dp[sub], sub);
-                    gather(x, dp[sub], sub);
+                }
+            } else {
+                const float apart_log2 = apart * kLog2e;
+#pragma unroll
+                for (int quad = 0; quad < 8; ++quad) {
+                    const f32x4 one = of(2, quad / 4, quad % 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 4 * (quad % 4) + j;
+                        s[quad / 4][r] = __builtin_fmaf(s[quad / 4][r], scale_log2, BIAS ? apart_log2 + one[j] : one[j]);
+                    }
                 }
             }
+#pragma unroll
+            for (int quad = 0; quad < 8; ++quad) {
+                const f32x4 e = of(3, quad / 4, quad % 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * (quad % 4) + j;
+                    s[quad / 4][r] = __builtin_amdgcn_exp2f(s[quad / 4][r]);
+                    dp[quad / 4][r] = s[quad / 4][r] * (dp[quad / 4][r] - e[j]);
+                }
+            }
+            between_runs();
+            gather(s, dp);
+            feed<8 * kParts, 2, 3>();
+            between_runs();
             if (more) store(now ^ 1);
             if constexpr (BIAS) {
                 if (turned && more) {  // another head's bias, once every wave is done with this one's
