@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
     for (int i = 0; i < kParts; ++i) o[i] = f32x16{};
     float top = -INFINITY, total = 0.f;
 
-    KeyWalk walk;
+    KeyWalk<kKeyTile> walk;
     walk.begin(a, b, split * a.tiles_per_split, (split + 1) * a.tiles_per_split);
     Copier<DP, kKeyTile, 256> ks, vs;
     ks.init(thread, a.k.middle, a.d);

@@ -157,17 +157,19 @@ __device__ __forceinline__ int row_length(const AttendArgs& a, int64_t row) {
     return min(max(uniform(a.lengths[row]), 0), a.length);
 }
 
-// Walks the key tiles (row, first, valid) with at least one key, of the places [begin, end) of passages x tiles.
+// Walks the tiles of KEYS keys that have at least one (of `row`, from `first` on; the row holds `count`), of the places
+// [begin, end) of passages x tiles.
+template <int KEYS>
 struct KeyWalk {
     int b, r, per_row, end, first, count;
     int64_t row;
 
     __device__ void begin(const AttendArgs& a, int batch, int place, int last) {
         b = batch;
-        per_row = (a.length + kKeyTile - 1) / kKeyTile;
+        per_row = (a.length + KEYS - 1) / KEYS;
         end = min(last, per_row * a.passages);
         r = place / max(per_row, 1);
-        first = (place - r * per_row) * kKeyTile;
+        first = (place - r * per_row) * KEYS;
         if (place < end) {
             row = bank_row(a, b, r);
             count = row_length(a, row);
@@ -176,9 +178,9 @@ struct KeyWalk {
             r = a.passages;
         }
     }
-    __device__ bool valid() const { return r * per_row + first / kKeyTile < end; }
+    __device__ bool valid() const { return r * per_row + first / KEYS < end; }
     __device__ void next(const AttendArgs& a) {
-        first += kKeyTile;
+        first += KEYS;
         settle(a);
     }
     __device__ void settle(const AttendArgs& a) {
