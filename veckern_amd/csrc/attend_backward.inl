@@ -97,20 +97,6 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     lse = make_float2(lse.x == -INFINITY ? INFINITY : lse.x, lse.y * -kLog2e);
 
     const float scale_log2 = a.scale * kLog2e;
-    int position = 0;
-    float below = 0.f, above = 0.f;
-    float *held = nullptr, *sums = nullptr, *skew = nullptr;
-    if constexpr (BIAS) {
-        const int places = bias_places(a.bias.far);
-        skew = shared + wave * kSkewFloats;
-        held = shared + 4 * kSkewFloats;
-        sums = held + (1 + wave) * places;
-        fill_bias<E>(a.bias, head, held, thread, 256);
-        for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
-        for (int i = thread; i < 4 * places; i += 256) held[places + i] = 0.f;
-        position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
-    }
-
     f32x16 dq[kParts];
 #pragma unroll
     for (int i = 0; i < kParts; ++i) dq[i] = f32x16{};
@@ -127,17 +113,35 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     };
     bool more = walk.valid();
     int now = 0;
+    if (more) load();  // before the biases: what they wait for is under way with it
+    int position = 0;
+    float below = 0.f, above = 0.f;
+    bool large = false;
+    float *held = nullptr, *sums = nullptr, *skew = nullptr;
+    if constexpr (BIAS) {
+        const int places = bias_places(a.bias.far);
+        skew = shared + wave * kSkewFloats;
+        held = shared + 4 * kSkewFloats;
+        sums = held + (1 + wave) * places;
+        large = fill_biases<E>(a.bias, head, 1, a.scale, held, thread, 256);
+        for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
+        for (int i = thread; i < 4 * places; i += 256) held[places + i] = 0.f;
+        position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
+    }
+
     if (more) {
-        load();
         ks.store(tile[0][0]);
         vs.store(tile[0][1]);
     }
     __syncthreads();
     const char *k, *v;
+    f32x16 rest;  // dP - delta begins with
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rest[r] = -delta;
     auto products = [&](f32x16 (&s)[kSubs], f32x16 (&dp)[kSubs]) {
 #pragma unroll
         for (int sub = 0; sub < kSubs; ++sub) {
-            s[sub] = dp[sub] = f32x16{};
+            dp[sub] = rest;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
@@ -153,68 +157,81 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 16 * half, i, lane), x, dq[i]);
         }
     };
-    while (more) {
-        const int first = walk.first, left = walk.count - walk.first;
-        walk.next(a);
-        more = walk.valid();
-        if (more) load();
-        k = tile[now][0];
-        v = tile[now][1];
-        bool near = false;  // the tile's keys do not share one bias
-        float apart = 0.f;
-        int t0 = 0;
-        if constexpr (BIAS) {
-            t0 = __builtin_amdgcn_readfirstlane(position);
-            apart = held[bias_index(a.bias.far, first - position)];
-            near = !far_apart(a.bias, first - (t0 + 31), first + kKeys - 1 - t0) || __any(fabsf(apart) > kLargeBias);
-        }
-        f32x16 s[kSubs], dp[kSubs];
-        between_runs();
-        products(s, dp);
-        feed<2 * kSubs * kSteps, 1, 4>();
-        between_runs();
-        if (BIAS && near) {
+    auto run = [&](auto kind) {
+        constexpr bool kLarge = decltype(kind)::value;
+        while (more) {
+            const int first = walk.first, left = walk.count - walk.first;
+            walk.next(a);
+            more = walk.valid();
+            if (more) load();
+            k = tile[now][0];
+            v = tile[now][1];
+            f32x16 s[kSubs] = {}, dp[kSubs];
+            bool near = kLarge;  // the tile's keys do not share one bias
+            float apart = 0.f;   // the bias they share
+            int t0 = 0;
+            if constexpr (BIAS) {
+                t0 = __builtin_amdgcn_readfirstlane(position);
+                if (!kLarge) {
+                    near = !far_apart(a.bias, first - (t0 + 31), first + kKeys - 1 - t0);
+                    if (near) {
 #pragma unroll
-            for (int sub = 0; sub < kSubs; ++sub) {
-                add_bias<1>(s[sub], a.scale, held, a.bias.far, first + 32 * sub + hi - position);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[sub][r] = __builtin_fmaf(s[sub][r] - lse.x, kLog2e, lse.y);
+                        for (int sub = 0; sub < kSubs; ++sub)
+                            each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position, [&](int r, float x) { s[sub][r] = x; });
+                    } else {
+                        apart = held[bias_index(a.bias.far, first - position)] * a.scale;
+                    }
+                }
             }
-        } else {
-            const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
+            between_runs();
+            products(s, dp);
+            feed<2 * kSubs * kSteps, 1, 4>();
+            between_runs();
+            if constexpr (kLarge) {
 #pragma unroll
-            for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_fmaf(s[r / 16][r % 16], scale_log2, shift);
-        }
-#pragma unroll
-        for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
-        if (left < kKeys) {
-#pragma unroll
-            for (int r = 0; r < 16 * kSubs; ++r)
-                if (r / 16 * 32 + tile_row(r % 16, hi) >= left) s[r / 16][r % 16] = 0.f;
-        }
-        if constexpr (BIAS) {
-            if (near) {
-#pragma unroll
-                for (int sub = 0; sub < kSubs; ++sub) add_by_distance(s[sub], skew, sums, a.bias.far, first + 32 * sub - t0, lane, below, above);
+                for (int sub = 0; sub < kSubs; ++sub)
+                    each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position, [&](int r, float x) {
+                        s[sub][r] = __builtin_fmaf(__builtin_fmaf(s[sub][r], a.scale, x) - lse.x, kLog2e, lse.y);
+                    });
             } else {
-                float all = 0.f;
+                const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
 #pragma unroll
-                for (int r = 0; r < 16 * kSubs; ++r) all += s[r / 16][r % 16];
-                if (first < position) below += all;
-                else above += all;
+                for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_fmaf(s[r / 16][r % 16], scale_log2, shift);
             }
+#pragma unroll
+            for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * dp[r / 16][r % 16];
+            if (left < kKeys) {
+#pragma unroll
+                for (int r = 0; r < 16 * kSubs; ++r)
+                    if (r / 16 * 32 + tile_row(r % 16, hi) >= left) s[r / 16][r % 16] = 0.f;
+            }
+            if constexpr (BIAS) {
+                if (near) {
+#pragma unroll
+                    for (int sub = 0; sub < kSubs; ++sub)
+                        add_by_distance(s[sub], skew, sums, a.bias.far, first + 32 * sub - t0, lane, below, above);
+                } else {
+                    float all = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16 * kSubs; ++r) all += s[r / 16][r % 16];
+                    if (first < position) below += all;
+                    else above += all;
+                }
+            }
+            between_runs();
+            gather(s);
+            feed<2 * kSubs * kParts, 2, 3>();
+            between_runs();
+            if (more) {
+                ks.store(tile[now ^ 1][0]);
+                vs.store(tile[now ^ 1][1]);
+            }
+            __syncthreads();
+            now ^= 1;
         }
-        between_runs();
-        gather(s);
-        feed<2 * kSubs * kParts, 2, 3>();
-        between_runs();
-        if (more) {
-            ks.store(tile[now ^ 1][0]);
-            vs.store(tile[now ^ 1][1]);
-        }
-        __syncthreads();
-        now ^= 1;
-    }
+    };
+    if (BIAS && large) run(std::integral_constant<bool, BIAS>());
+    else run(std::false_type());
 
     if (used) {
         char* out = static_cast<char*>(g.d_q.p) + at(g.d_q) * 2;
@@ -263,8 +280,8 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = 64;
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kQueries>];
-    // of each query, in the order of the products' rows: lse and -what its rounding left off * log2(e); both as one in log2
-    // units, negative; delta
+    // of each query, in the order of the products' rows: -lse / scale and -delta, with which the products' sums begin; for
+    // large biases lse and -what its rounding left off * log2(e)
     __shared__ __align__(16) float stat[2][4][kQueries];
     extern __shared__ float bias_held[];
 
@@ -294,7 +311,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                 vf[i] = column(a.v, v, there, i, hi, a.d);
             }
         }
-        const float scale_log2 = a.scale * kLog2e;
+        const float scale_log2 = a.scale * kLog2e, by_scale = 1.f / a.scale;
         const int start = BIAS ? a.q_start_all + (a.q_start ? uniform(a.q_start[b]) : 0) : 0;
         Copier<DP, kQueries, 256> qs, ds;
         qs.init(thread, a.q.middle, a.d);
@@ -319,14 +336,19 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
             if (thread < kQueries) {
                 const int at = place_of(thread);
                 const float value = lse.x == -INFINITY ? INFINITY : lse.x, low = lse.y * -kLog2e;
-                stat[to][0][at] = value;
-                stat[to][1][at] = low;
-                stat[to][2][at] = __builtin_fmaf(value, -kLog2e, low);
-                stat[to][3][at] = delta;
+                stat[to][0][at] = (low * kLn2 - value) * by_scale;
+                stat[to][1][at] = -delta;
+                stat[to][2][at] = value;
+                stat[to][3][at] = low;
             }
         };
         load();
-        if constexpr (BIAS) fill_bias<E>(a.bias, head, bias_held, thread, 256);
+        bool large = false;
+        if constexpr (BIAS) {
+            large = share > 1 && large_bias<E>(a.bias, head, share, a.scale, thread, 256);
+            if (large) fill_bias<E>(a.bias, head, 1.f, bias_held, thread, 256);
+            else large = fill_biases<E>(a.bias, head, 1, a.scale, bias_held, thread, 256);
+        }
         store(0);
         __syncthreads();
         int now = 0;
@@ -338,7 +360,6 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         auto products = [&](f32x16 (&s)[2], f32x16 (&dp)[2]) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-                s[sub] = dp[sub] = f32x16{};
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
                     s[sub] = E::mfma(straight<DP>(q, 32 * sub, i, lane), kf[i], s[sub]);
@@ -357,80 +378,83 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                 }
             }
         };
-        while (more) {
-            const int from = first;
-            first += kQueries;
-            bool turned = false;
-            if (first >= a.tokens) {
-                first = 0;
-                ++head;
-                turned = true;
-            }
-            more = head < (kv_head + 1) * share;
-            if (more) load();
-            q = tile[now][0];
-            d = tile[now][1];
-            bool near = false;  // the tile's places do not share one bias
-            float apart = 0.f;
-            if constexpr (BIAS) {
-                const int k0 = key_tile * kColumns + wave * 32;
-                apart = bias_held[bias_index(a.bias.far, key - (from + start))];
-                near = !far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start)) ||
-                       __any(fabsf(apart) > kLargeBias);
-            }
-            f32x16 s[2], dp[2];
-            between_runs();
-            products(s, dp);
-            feed<4 * kSteps, 1, 4>();
-            between_runs();
-            if (BIAS && near) {
-#pragma unroll
-                for (int sub = 0; sub < 2; ++sub) {
-                    add_bias<-1>(s[sub], a.scale, bias_held, a.bias.far, key - (from + start + 32 * sub + hi));
-#pragma unroll
-                    for (int quad = 0; quad < 4; ++quad) {
-                        const f32x4 l = of(0, sub, quad), low = of(1, sub, quad);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            s[sub][4 * quad + j] = __builtin_fmaf(s[sub][4 * quad + j] - l[j], kLog2e, low[j]);
-                    }
+        auto run = [&](auto kind) {
+            constexpr bool kLarge = decltype(kind)::value;
+            while (more) {
+                const int from = first;
+                first += kQueries;
+                bool turned = false;
+                if (first >= a.tokens) {
+                    first = 0;
+                    ++head;
+                    turned = true;
                 }
-            } else {
-                const float apart_log2 = apart * kLog2e;
+                more = head < (kv_head + 1) * share;
+                if (more) load();
+                q = tile[now][0];
+                d = tile[now][1];
+                f32x16 s[2], dp[2];
 #pragma unroll
                 for (int quad = 0; quad < 8; ++quad) {
-                    const f32x4 one = of(2, quad / 4, quad % 4);
+                    const f32x4 l = of(0, quad / 4, quad % 4), e = of(1, quad / 4, quad % 4);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * (quad % 4) + j;
-                        s[quad / 4][r] = __builtin_fmaf(s[quad / 4][r], scale_log2, BIAS ? apart_log2 + one[j] : one[j]);
+                        s[quad / 4][4 * (quad % 4) + j] = kLarge ? 0.f : l[j];
+                        dp[quad / 4][4 * (quad % 4) + j] = e[j];
                     }
                 }
-            }
+                float apart = 0.f;  // a bias that all places of the tile share
+                if constexpr (BIAS && !kLarge) {
+                    const int k0 = key_tile * kColumns + wave * 32;
+                    if (far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start))) {
+                        apart = bias_held[bias_index(a.bias.far, key - (from + start))] * scale_log2;
+                    } else {
 #pragma unroll
-            for (int quad = 0; quad < 8; ++quad) {
-                const f32x4 e = of(3, quad / 4, quad % 4);
+                        for (int sub = 0; sub < 2; ++sub)
+                            each_bias<-1>(bias_held, a.bias.far, key - (from + start + 32 * sub + hi),
+                                          [&](int r, float x) { s[sub][r] += x; });
+                    }
+                }
+                between_runs();
+                products(s, dp);
+                feed<4 * kSteps, 1, 4>();
+                between_runs();
+                if constexpr (kLarge) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * (quad % 4) + j;
-                    s[quad / 4][r] = __builtin_amdgcn_exp2f(s[quad / 4][r]);
-                    dp[quad / 4][r] = s[quad / 4][r] * (dp[quad / 4][r] - e[j]);
+                    for (int sub = 0; sub < 2; ++sub) {
+                        each_bias<-1>(bias_held, a.bias.far, key - (from + start + 32 * sub + hi),
+                                      [&](int r, float x) { s[sub][r] = __builtin_fmaf(s[sub][r], a.scale, x); });
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            s[sub][r] = __builtin_fmaf(s[sub][r] - of(2, sub, r / 4)[r % 4], kLog2e, of(3, sub, r / 4)[r % 4]);
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r)
+                        s[r / 16][r % 16] = BIAS ? __builtin_fmaf(s[r / 16][r % 16], scale_log2, apart) : s[r / 16][r % 16] * scale_log2;
                 }
-            }
-            between_runs();
-            gather(s, dp);
-            feed<8 * kParts, 2, 3>();
-            between_runs();
-            if (more) store(now ^ 1);
-            if constexpr (BIAS) {
-                if (turned && more) {  // another head's bias, once every wave is done with this one's
-                    __syncthreads();
-                    fill_bias<E>(a.bias, head, bias_held, thread, 256);
+#pragma unroll
+                for (int r = 0; r < 32; ++r) {
+                    s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]);
+                    dp[r / 16][r % 16] *= s[r / 16][r % 16];
                 }
+                between_runs();
+                gather(s, dp);
+                feed<8 * kParts, 2, 3>();
+                between_runs();
+                if (more) store(now ^ 1);
+                if constexpr (BIAS) {
+                    if (turned && more) {  // another head's bias, once every wave is done with this one's
+                        __syncthreads();
+                        fill_bias<E>(a.bias, head, kLarge ? 1.f : by_scale, bias_held, thread, 256);
+                    }
+                }
+                __syncthreads();
+                now ^= 1;
             }
-            __syncthreads();
-            now ^= 1;
-        }
+        };
+        if (BIAS && large) run(std::integral_constant<bool, BIAS>());
+        else run(std::false_type());
     }
 
     if (key < a.length) {  // keys past the row's length have no gradient: zeros
@@ -460,8 +484,8 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[3][2][kTileBytes<DP, kQueries>];
     __shared__ f32x4 handed[2][4][4][64];  // P of a tile: by waves, quads of rows, lanes
-    // of each query, in the order of the products' rows: lse and -what its rounding left off * log2(e); both as one in log2
-    // units, negative; delta
+    // of each query, in the order of the products' rows: -lse / scale and -delta, with which the products' sums begin; for
+    // large biases lse and -what its rounding left off * log2(e)
     __shared__ __align__(16) float stat[3][4][kQueries];
     extern __shared__ float bias_held[];
 
@@ -489,7 +513,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) own[i] = column(v, at, there, i, hi, a.d);
         }
-        const float scale_log2 = a.scale * kLog2e;
+        const float scale_log2 = a.scale * kLog2e, by_scale = 1.f / a.scale;
         const int start = BIAS ? a.q_start_all + (a.q_start ? uniform(a.q_start[b]) : 0) : 0;
         const int query_tiles = (a.tokens + kQueries - 1) / kQueries, tiles = query_tiles * share;
         const AttendView& rows = second ? g.d_out : a.q;  // each half of the block copies one of the two
@@ -512,14 +536,14 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
             if (thread < kQueries) {
                 const int at = place_of(thread);
                 const float value = lse.x == -INFINITY ? INFINITY : lse.x, low = lse.y * -kLog2e;
-                stat[to][0][at] = value;
-                stat[to][1][at] = low;
-                stat[to][2][at] = __builtin_fmaf(value, -kLog2e, low);
-                stat[to][3][at] = delta;
+                stat[to][0][at] = (low * kLn2 - value) * by_scale;
+                stat[to][1][at] = -delta;
+                stat[to][2][at] = value;
+                stat[to][3][at] = low;
             }
         };
-        auto products = [&](const char* rows) {
-            f32x16 s{};
+        auto products = [&](f32x16 s, const char* rows) {
+            between_runs();
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(rows, 0, i, lane), own[i], s);
             feed<kSteps, 1, 4>();
@@ -538,12 +562,17 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         };
         int head = kv_head * share, first = 0;  // of the tile that is loaded next
         load(head, first);
-        if constexpr (BIAS) fill_bias<E>(a.bias, head, bias_held, thread, 512);
+        bool large = false;
+        if constexpr (BIAS) {
+            large = share > 1 && large_bias<E>(a.bias, head, share, a.scale, thread, 512);
+            if (large) fill_bias<E>(a.bias, head, 1.f, bias_held, thread, 512);
+            else large = fill_biases<E>(a.bias, head, 1, a.scale, bias_held, thread, 512);
+        }
         store(0);
         __syncthreads();
         // each half of the block has a loop of its own, with the same barriers
-        auto run = [&](auto half) {
-            constexpr bool kSecond = decltype(half)::value;
+        auto run = [&](auto half, auto kind) {
+            constexpr bool kSecond = decltype(half)::value, kLarge = decltype(kind)::value;
             int now = 0, before = 2, from = 0;
             for (int n = 0; n <= tiles; ++n) {
                 const int after = now == 2 ? 0 : now + 1;
@@ -556,35 +585,31 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                 }
                 if (n + 1 < tiles) load(head, first);
                 between_runs();
+                auto begin = [&](int at, int which) {
+                    f32x16 x;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[r] = reinterpret_cast<const f32x4*>(&stat[at][which][mfma_row(r / 4 * 4, hi)])[0][r % 4];
+                    return x;
+                };
                 if (!kSecond && n < tiles) {
-                    f32x16 s = products(tile[now][0]);
-                    auto of = [&](int which, int quad) {
-                        return *reinterpret_cast<const f32x4*>(&stat[now][which][mfma_row(4 * quad, hi)]);
-                    };
-                    bool near = false;  // the tile's places do not share one bias
-                    float apart = 0.f;
-                    if constexpr (BIAS) {
-                        apart = bias_held[bias_index(a.bias.far, key - (from + start))];
-                        near = !far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start)) ||
-                               __any(fabsf(apart) > kLargeBias);
+                    f32x16 s = kLarge ? f32x16{} : begin(now, 0);
+                    float apart = 0.f;  // a bias that all places of the tile share
+                    if constexpr (BIAS && !kLarge) {
+                        if (far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start))) {
+                            apart = bias_held[bias_index(a.bias.far, key - (from + start))] * scale_log2;
+                        } else {
+                            each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), [&](int r, float x) { s[r] += x; });
+                        }
                     }
-                    if (BIAS && near) {
-                        add_bias<-1>(s, a.scale, bias_held, a.bias.far, key - (from + start + hi));
-#pragma unroll
-                        for (int quad = 0; quad < 4; ++quad) {
-                            const f32x4 l = of(0, quad), low = of(1, quad);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) s[4 * quad + j] = __builtin_fmaf(s[4 * quad + j] - l[j], kLog2e, low[j]);
-                        }
+                    s = products(s, tile[now][0]);
+                    if constexpr (kLarge) {
+                        const f32x16 l = begin(now, 2), low = begin(now, 3);
+                        each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), [&](int r, float x) {
+                            s[r] = __builtin_fmaf(__builtin_fmaf(s[r], a.scale, x) - l[r], kLog2e, low[r]);
+                        });
                     } else {
-                        const float apart_log2 = apart * kLog2e;
 #pragma unroll
-                        for (int quad = 0; quad < 4; ++quad) {
-                            const f32x4 one = of(2, quad);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                s[4 * quad + j] = __builtin_fmaf(s[4 * quad + j], scale_log2, BIAS ? apart_log2 + one[j] : one[j]);
-                        }
+                        for (int r = 0; r < 16; ++r) s[r] = BIAS ? __builtin_fmaf(s[r], scale_log2, apart) : s[r] * scale_log2;
                     }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
@@ -593,13 +618,12 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                         handed[n % 2][wave][quad][lane] = f32x4{s[4 * quad], s[4 * quad + 1], s[4 * quad + 2], s[4 * quad + 3]};
                     gather(s, tile[now][1]);
                 } else if (kSecond && n > 0) {
-                    f32x16 dp = products(tile[before][1]);
+                    f32x16 dp = products(begin(before, 1), tile[before][1]);
 #pragma unroll
                     for (int quad = 0; quad < 4; ++quad) {
                         const f32x4 p = handed[(n + 1) % 2][wave][quad][lane];
-                        const f32x4 e = *reinterpret_cast<const f32x4*>(&stat[before][3][mfma_row(4 * quad, hi)]);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) dp[4 * quad + j] = p[j] * (dp[4 * quad + j] - e[j]);
+                        for (int j = 0; j < 4; ++j) dp[4 * quad + j] *= p[j];
                     }
                     gather(dp, tile[before][0]);
                 }
@@ -608,7 +632,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                 if constexpr (BIAS) {
                     if (turned && n + 1 < tiles) {  // another head's bias, once every wave is done with this one's
                         __syncthreads();
-                        fill_bias<E>(a.bias, head, bias_held, thread, 512);
+                        fill_bias<E>(a.bias, head, kLarge ? 1.f : by_scale, bias_held, thread, 512);
                     }
                 }
                 __syncthreads();
@@ -616,8 +640,12 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                 now = after;
             }
         };
-        if (second) run(std::true_type());
-        else run(std::false_type());
+        auto both = [&](auto kind) {
+            if (second) run(std::true_type(), kind);
+            else run(std::false_type(), kind);
+        };
+        if (BIAS && large) both(std::integral_constant<bool, BIAS>());
+        else both(std::false_type());
     }
 
     if (key < a.length) {  // keys past the row's length have no gradient: zeros

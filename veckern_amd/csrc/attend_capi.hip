@@ -71,6 +71,7 @@ AttendBias bias_of(size_t buckets, size_t max_distance, bool two_sided) {
         const long double whole = std::round(x);
         s.edge[i - 1] = static_cast<int>(std::fabs(x - whole) < 1e-12L * x ? whole : std::ceil(x));
     }
+    for (int i = s.edges; i < vk::kMostEdges; ++i) s.edge[i] = INT32_MAX;
     s.far = s.edges ? s.edge[s.edges - 1] : e;
     return s;
 }

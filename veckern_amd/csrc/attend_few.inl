@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
     if constexpr (BIAS) {
         float* all = reinterpret_cast<float*>(shared + kFewTiles<DP> + kFewPassages * sizeof(int2));
         const int places = bias_places(a.bias.far);
-        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, all + p * places, thread, kThreads);
+        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, 1.f, all + p * places, thread, kThreads);
         held = all + (head - group * a.pack) * places;
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(mine, 0, i, lane), qf[i], s);
         if constexpr (BIAS) {
-            add_bias<1>(s, a.scale, held, a.bias.far, from - position + hi);
+            each_bias<1>(held, a.bias.far, from - position + hi, [&](int i, float x) { s[i] = __builtin_fmaf(s[i], a.scale, x); });
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= a.scale;

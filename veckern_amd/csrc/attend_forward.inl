@@ -9,6 +9,8 @@
 // normalises it, the maximum and the output are held in 32 bits. The weights are relative to a maximum that is only raised
 // when it grew by more than kSlack: the output's rescaling is rare, and P <= e^kSlack keeps its relative precision in either
 // type.
+#include <type_traits>
+
 #include "attend_tile.hpp"
 
 namespace vk::attend {
@@ -37,15 +39,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
 
-    const float* held = nullptr;
-    int position = 0;
-    if constexpr (BIAS) {
-        const int places = bias_places(a.bias.far);
-        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, bias_held + p * places, thread, 256);
-        held = bias_held + (head - group * a.pack) * places;
-        position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
-    }
-
     f32x16 o[kParts];
 #pragma unroll
     for (int i = 0; i < kParts; ++i) o[i] = f32x16{};
@@ -63,98 +56,106 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
     };
     bool more = walk.valid();
     int now = 0;
+    if (more) load();  // before the biases: what they wait for is under way with it
+    const float* held = nullptr;
+    int position = 0;
+    bool large = false;
+    if constexpr (BIAS) {
+        large = fill_biases<E>(a.bias, group * a.pack, a.pack, a.scale, bias_held, thread, 256);
+        held = bias_held + (head - group * a.pack) * bias_places(a.bias.far);
+        position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
+    }
     if (more) {
-        load();
         ks.store(tile[0][0]);
         vs.store(tile[0][1]);
     }
     __syncthreads();
-    while (more) {
-        const int first = walk.first, left = walk.count - walk.first;
-        walk.next(a);
-        more = walk.valid();
-        if (more) load();
+    auto run = [&](auto kind) {
+        constexpr bool kLarge = decltype(kind)::value;
+        while (more) {
+            const int first = walk.first, left = walk.count - walk.first;
+            walk.next(a);
+            more = walk.valid();
+            if (more) load();
 
-        f32x16 s[2];
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            s[sub] = f32x16{};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), qf[i], s[sub]);
-        }
-        feed<2 * kSteps, 1, 4>();
-        __builtin_amdgcn_sched_barrier(0);
-        bool near = false;
-        float apart = 0.f;
-        if constexpr (BIAS) {
-            const int x0 = first - position;
-            // the wave's tokens lie between its first and last column's
-            const int t0 = __builtin_amdgcn_readfirstlane(position), t1 = __builtin_amdgcn_readlane(position, 31);
-            near = !far_apart(a.bias, first - t1, first + kKeyTile - 1 - t0);
-            if (near) {
-#pragma unroll
-                for (int sub = 0; sub < 2; ++sub) add_bias<1>(s[sub], a.scale, held, a.bias.far, x0 + 32 * sub + hi);
-            } else {
-                apart = held[bias_index(a.bias.far, x0)];
-                if (__any(fabsf(apart) > kLargeBias)) {
+            f32x16 s[2] = {};
+            float apart = 0.f;  // a bias that all keys of the tile share
+            if constexpr (BIAS && !kLarge) {
+                // the wave's tokens lie between its first and last column's
+                const int t0 = __builtin_amdgcn_readfirstlane(position), t1 = __builtin_amdgcn_readlane(position, 31);
+                if (far_apart(a.bias, first - t1, first + kKeyTile - 1 - t0)) {
+                    apart = held[bias_index(a.bias.far, first - position)] * a.scale;
+                } else {
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) s[sub][r] = __builtin_fmaf(s[sub][r], a.scale, apart);
-                    near = true;
+                        each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position, [&](int r, float x) { s[sub][r] = x; });
                 }
             }
-        }
-        if (left < kKeyTile) {
+            __builtin_amdgcn_s_setprio(1);
+            between_runs();
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (32 * sub + tile_row(r, hi) >= left) s[sub][r] = -INFINITY;
-        }
-        // where all keys share one bias s stays the plain product, and scale and bias go into the exponent's one step
-        float most = s[0][0];
+                for (int i = 0; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), qf[i], s[sub]);
+            feed<2 * kSteps, 1, 4>();
+            between_runs();
+            __builtin_amdgcn_s_setprio(0);
+            if constexpr (kLarge) {
 #pragma unroll
-        for (int r = 1; r < 32; ++r) most = fmaxf(most, s[r / 16][r % 16]);
-        most = both_max(most);
-        if (!near && most != -INFINITY) most = __builtin_fmaf(most, a.scale, apart);
-        if (__any(most > top + kSlack)) {
-            const float raised = fmaxf(top, most);
-            const float factor = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - raised) * kLog2e);
-            top = raised;
-            total *= factor;
+                for (int sub = 0; sub < 2; ++sub)
+                    each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position,
+                                 [&](int r, float x) { s[sub][r] = __builtin_fmaf(s[sub][r], a.scale, x); });
+            }
+            if (left < kKeyTile) {
 #pragma unroll
-            for (int i = 0; i < kParts; ++i)
+                for (int r = 0; r < 32; ++r)
+                    if (r / 16 * 32 + tile_row(r % 16, hi) >= left) s[r / 16][r % 16] = -INFINITY;
+            }
+            float most = s[0][0];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[i][r] *= factor;
-        }
-        const float base = top == -INFINITY ? 0.f : top;
-        if (BIAS && near) {
+            for (int r = 1; r < 32; ++r) most = fmaxf(most, s[r / 16][r % 16]);
+            most = both_max(most);
+            if (!kLarge) most = __builtin_fmaf(most, a.scale, apart);
+            if (__any(most > top + kSlack)) {
+                const float raised = fmaxf(top, most);
+                const float factor = raised == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((top - raised) * kLog2e);
+                top = raised;
+                total *= factor;
 #pragma unroll
-            for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f((s[r / 16][r % 16] - base) * kLog2e);
-        } else {
+                for (int i = 0; i < kParts; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[i][r] *= factor;
+            }
+            const float base = top == -INFINITY ? 0.f : top;
+            // scale, shared bias and maximum go into the exponent's one step
             const float by = a.scale * kLog2e, shift = (apart - base) * kLog2e;
 #pragma unroll
-            for (int r = 0; r < 32; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r / 16][r % 16], by, shift));
-        }
+            for (int r = 0; r < 32; ++r) {
+                const float x = s[r / 16][r % 16];
+                s[r / 16][r % 16] = __builtin_amdgcn_exp2f(kLarge ? (x - base) * kLog2e : __builtin_fmaf(x, by, shift));
+                total += s[r / 16][r % 16];
+            }
+            __builtin_amdgcn_s_setprio(1);
+            between_runs();
 #pragma unroll
-        for (int r = 0; r < 32; ++r) total += s[r / 16][r % 16];
-        __builtin_amdgcn_sched_barrier(0);
+            for (int half = 0; half < 4; ++half) {
+                const s16x8 p = rounded<E>(s[half / 2], half % 2);
 #pragma unroll
-        for (int step = 0; step < 4; ++step) {
-            const s16x8 p = rounded<E>(s[step / 2], step % 2);
-#pragma unroll
-            for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(tile[now][1], 16 * step, i, lane), p, o[i]);
+                for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(tile[now][1], 16 * half, i, lane), p, o[i]);
+            }
+            feed<4 * kParts, 2, 4>();
+            between_runs();
+            __builtin_amdgcn_s_setprio(0);
+            if (more) {
+                ks.store(tile[now ^ 1][0]);
+                vs.store(tile[now ^ 1][1]);
+            }
+            __syncthreads();
+            now ^= 1;
         }
-        feed<4 * kParts, 2, 4>();
-        __builtin_amdgcn_sched_barrier(0);
-        if (more) {
-            ks.store(tile[now ^ 1][0]);
-            vs.store(tile[now ^ 1][1]);
-        }
-        __syncthreads();
-        now ^= 1;
-    }
+    };
+    if (BIAS && large) run(std::integral_constant<bool, BIAS>());
+    else run(std::false_type());
 
     total = both_sum(total);
     if (!used) return;

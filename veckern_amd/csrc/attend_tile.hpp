@@ -208,46 +208,67 @@ __device__ __forceinline__ int bias_places(int far) { return 2 * far + 2 * kPad 
 __device__ __forceinline__ int bias_index(int far, int x) { return min(max(x + far + kPad, 0), 2 * far + kPad); }
 __device__ __forceinline__ int bucket_of(const AttendBias& s, int x) {
     const int a = s.two_sided ? abs(x) : max(-x, 0), exact = s.side / 2;
-    int bucket = a;
-    if (a >= exact) {
-        int lo = 0, hi = s.edges;  // the number of edges <= a
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (s.edge[mid] <= a) lo = mid + 1;
-            else hi = mid;
-        }
-        bucket = exact + lo;
+    int beyond = exact;
+    for (int i = 0; i < s.edges; i += 16) {  // the edges come through scalar registers; those past the last are out of reach
+#pragma unroll
+        for (int j = 0; j < 16; ++j) beyond += s.edge[i + j] <= a;
     }
+    const int bucket = a < exact ? a : beyond;
     return bucket + (s.two_sided && x > 0 ? s.side : 0);
 }
 template <class E>
-__device__ __forceinline__ void fill_bias(const AttendBias& s, int head, float* held, int thread, int threads) {
-    for (int i = thread; i < bias_places(s.far); i += threads) {
-        const auto* t = static_cast<const typename E::T*>(s.table);
-        held[i] = static_cast<float>(t[bucket_of(s, i - s.far - kPad) * s.bucket_stride + head * s.head_stride]);
-    }
+__device__ __forceinline__ float bias_at(const AttendBias& s, int head, int place) {
+    const auto* t = static_cast<const typename E::T*>(s.table);
+    return static_cast<float>(t[bucket_of(s, place - s.far - kPad) * s.bucket_stride + head * s.head_stride]);
+}
+template <class E>
+__device__ __forceinline__ void fill_bias(const AttendBias& s, int head, float factor, float* held, int thread, int threads) {
+    for (int i = thread; i < bias_places(s.far); i += threads) held[i] = bias_at<E>(s, head, i) * factor;
+}
+// Where a logit is scale * product + bias, the product's sum can begin with bias / scale, so that adding the bias costs no
+// instruction. That is not so where a bias is so large that it swallows what is added to it (a type's lowest value, say, for
+// "almost never"), or the scale so small that the quotient overflows: then the bias is added to each scaled product, as the
+// definition does. The same for all threads of the block.
+__device__ __forceinline__ bool is_large(float bias) { return fabsf(bias) > 1e4f && !isinf(bias); }
+template <class E>
+__device__ __forceinline__ bool large_bias(const AttendBias& s, int head, int heads, float scale, int thread, int threads) {
+    const auto* t = static_cast<const typename E::T*>(s.table);
+    bool large = scale < 1e-20f;
+    for (int i = thread; i < s.buckets * heads; i += threads)
+        large = large || is_large(static_cast<float>(t[i / heads * s.bucket_stride + (head + i % heads) * s.head_stride]));
+    return __syncthreads_or(large);
+}
+// Both at once for `heads` heads, one behind the other: biases divided by the scale, or, where true is returned, as they are.
+template <class E>
+__device__ __forceinline__ bool fill_biases(const AttendBias& s, int head, int heads, float scale, float* held, int thread, int threads) {
+    const int places = bias_places(s.far);
+    bool large = scale < 1e-20f;
+    for (int h = 0; h < heads; ++h)
+        for (int i = thread; i < places; i += threads) {
+            const float x = bias_at<E>(s, head + h, i);
+            large = large || is_large(x);
+            held[h * places + i] = x;
+        }
+    large = __syncthreads_or(large);
+    if (!large)
+        for (int h = 0; h < heads; ++h)
+            for (int i = thread; i < places; i += threads) held[h * places + i] *= 1.f / scale;  // a thread's own
+    return large;
 }
 // Whether all distances in [least, most] share one bucket of the far ends (one-sided: all that are not negative do too).
 __device__ __forceinline__ bool far_apart(const AttendBias& s, int least, int most) {
     return most <= -s.far || least >= (s.two_sided ? s.far : 0);
 }
 
-// A bias beyond this swallows what is added to it in part or whole: it is added to each product first, as the definition
-// does, also where a tile's keys share one.
-constexpr float kLargeBias = 1e4f;
-
-// The logits of a 32 x 32 tile, scores * scale + bias, in natural units (a type's lowest value, as a bias that almost never
-// lets a key through, would overflow in log2 units). x0: the distance at tile_row(0, hi) of the lane; STEP: how it changes
-// from row to row.
-template <int STEP>
-__device__ __forceinline__ void add_bias(f32x16& s, float scale, const float* held, int far, int x0) {
+// The biases of a 32 x 32 tile. x0: the distance at tile_row(0, hi) of the lane; STEP: how it changes from row to row.
+template <int STEP, class F>
+__device__ __forceinline__ void each_bias(const float* held, int far, int x0, F&& use) {
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         const int x = x0 + STEP * 16 * part;
         const float* at = held + bias_index(far, STEP > 0 ? x : x - 14);
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-            s[8 * part + r] = __builtin_fmaf(s[8 * part + r], scale, at[STEP > 0 ? tile_row(r, 0) : 14 - tile_row(r, 0)]);
+        for (int r = 0; r < 8; ++r) use(8 * part + r, at[STEP > 0 ? tile_row(r, 0) : 14 - tile_row(r, 0)]);
     }
 }
 
