@@ -23,26 +23,26 @@ __device__ __forceinline__ void store_four(void* p, int at, const f32x16& x, int
 // Adds dS of a 32 x 32 tile (lane: one query position, x: the distance of the tile's first key from the first query) to a
 // wave's sums by distance, in a fixed order. The tile goes through LDS by diagonals: element (key, query) to row 31 + key -
 // query and place `query` of `skew`, whose other places stay zero; then a lane sums one diagonal and adds it to that distance's
-// place, or, beyond the far ends, to a register. With 36 floats a row neither the writes nor the 16-byte reads share a bank.
-// (Adding each element to its distance's place by an LDS atomic took 130 clocks an instruction.)
+// place, or, beyond the far ends, to a register. With 36 floats a row neither the writes nor the 16-byte reads share a bank. The
+// two steps are apart so that products run between them. (Adding each element to its distance's place by an LDS atomic took 130
+// clocks an instruction.)
 constexpr int kSkew = 36, kSkewFloats = 63 * kSkew;
-__device__ __forceinline__ void add_by_distance(const f32x16& ds, float* skew, float* sums, int far, int x, int lane, float& below,
-                                                float& above) {
+__device__ __forceinline__ void put_diagonals(const f32x16& ds, float* skew, int lane) {
     float* to = skew + (31 - lane % 32 + lane / 32) * kSkew + lane % 32;
 #pragma unroll
     for (int r = 0; r < 16; ++r) to[tile_row(r, 0) * kSkew] = ds[r];
     between_lanes();
-    if (lane < 63) {
-        const f32x4* from = reinterpret_cast<const f32x4*>(skew + lane * kSkew);
-        f32x4 y = from[0];
+}
+__device__ __forceinline__ void sum_diagonals(const float* skew, float* sums, int far, int x, int lane, float& below, float& above) {
+    const f32x4* from = reinterpret_cast<const f32x4*>(skew + min(lane, 62) * kSkew);
+    f32x4 y = from[0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) y += from[i];
-        const float all = (y[0] + y[1]) + (y[2] + y[3]);
-        const int place = x + lane - 31 + far + kPad;
-        if (place < 0) below += all;
-        else if (place > 2 * far + 2 * kPad) above += all;
-        else sums[place] += all;
-    }
+    for (int i = 1; i < 8; ++i) y += from[i];
+    const float all = lane < 63 ? (y[0] + y[1]) + (y[2] + y[3]) : 0.f;
+    const int place = x + lane - 31 + far + kPad;
+    if (place < 0) below += all;
+    else if (place > 2 * far + 2 * kPad) above += all;
+    else if (lane < 63) sums[place] += all;
     between_lanes();
 }
 
@@ -135,13 +135,9 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     }
     __syncthreads();
     const char *k, *v;
-    f32x16 rest;  // dP - delta begins with
-#pragma unroll
-    for (int r = 0; r < 16; ++r) rest[r] = -delta;
     auto products = [&](f32x16 (&s)[kSubs], f32x16 (&dp)[kSubs]) {
 #pragma unroll
         for (int sub = 0; sub < kSubs; ++sub) {
-            dp[sub] = rest;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
@@ -149,13 +145,16 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             }
         }
     };
-    auto gather = [&](const f32x16 (&ds)[kSubs]) {
+    auto gather = [&](const f32x16& ds, int sub) {
+        between_runs();
 #pragma unroll
-        for (int half = 0; half < 2 * kSubs; ++half) {
-            const s16x8 x = rounded<E>(ds[half / 2], half % 2);
+        for (int half = 0; half < 2; ++half) {
+            const s16x8 x = rounded<E>(ds, half);
 #pragma unroll
-            for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 16 * half, i, lane), x, dq[i]);
+            for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 32 * sub + 16 * half, i, lane), x, dq[i]);
         }
+        feed<2 * kParts, 2, 3>();
+        between_runs();
     };
     auto run = [&](auto kind) {
         constexpr bool kLarge = decltype(kind)::value;
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             if (more) load();
             k = tile[now][0];
             v = tile[now][1];
-            f32x16 s[kSubs] = {}, dp[kSubs];
+            f32x16 s[kSubs] = {}, dp[kSubs] = {};
             bool near = kLarge;  // the tile's keys do not share one bias
             float apart = 0.f;   // the bias they share
             int t0 = 0;
@@ -199,7 +198,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
                 for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_fmaf(s[r / 16][r % 16], scale_log2, shift);
             }
 #pragma unroll
-            for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * dp[r / 16][r % 16];
+            for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
             if (left < kKeys) {
 #pragma unroll
                 for (int r = 0; r < 16 * kSubs; ++r)
@@ -207,9 +206,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             }
             if constexpr (BIAS) {
                 if (near) {
-#pragma unroll
-                    for (int sub = 0; sub < kSubs; ++sub)
-                        add_by_distance(s[sub], skew, sums, a.bias.far, first + 32 * sub - t0, lane, below, above);
+                    put_diagonals(s[0], skew, lane);
                 } else {
                     float all = 0.f;
 #pragma unroll
@@ -218,10 +215,15 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
                     else above += all;
                 }
             }
-            between_runs();
-            gather(s);
-            feed<2 * kSubs * kParts, 2, 3>();
-            between_runs();
+            gather(s[0], 0);
+#pragma unroll
+            for (int sub = 1; sub <= kSubs; ++sub) {
+                if (BIAS && near) {
+                    sum_diagonals(skew, sums, a.bias.far, first + 32 * (sub - 1) - t0, lane, below, above);
+                    if (sub < kSubs) put_diagonals(s[sub], skew, lane);
+                }
+                if (sub < kSubs) gather(s[sub], sub);
+            }
             if (more) {
                 ks.store(tile[now ^ 1][0]);
                 vs.store(tile[now ^ 1][1]);
