@@ -45,7 +45,7 @@ def test_missing_tensors_and_workspaces_are_refused():
     assert lib.vk_attend(None, None, 0, None) == invalid
     assert lib.vk_attend_workspace(ctypes.byref(arguments()), None) == invalid
     assert lib.vk_bias_bucket(1, 32, 128, 1, None) == invalid
-    a = arguments(tokens=40)  # few blocks and several tiles of keys: their parts are joined in a workspace
+    a = arguments()
     assert lib.vk_attend(ctypes.byref(a), None, 0, None) == invalid and b"q is NULL" in lib.vk_last_error()
     # host addresses that are never read: the call is refused before a launch
     held = (ctypes.c_char * 4096)()
@@ -63,8 +63,6 @@ def test_missing_tensors_and_workspaces_are_refused():
     a.q.data = base + 8
     assert lib.vk_attend(ctypes.byref(a), None, 0, None) == invalid and b"aligned" in lib.vk_last_error()
     a.q.data = base
-    assert lib.vk_attend_workspace(ctypes.byref(a), ctypes.byref(size)) == vk.VK_OK and size.value > 0
-    assert lib.vk_attend(ctypes.byref(a), None, 0, None) == invalid and b"workspace" in lib.vk_last_error()
     assert lib.vk_attend_backward(ctypes.byref(a), None, None, 0, None) == invalid
     g = vk._AttentionGrad()
     for t in (g.d_out, g.d_q, g.d_k, g.d_v):
@@ -74,5 +72,8 @@ def test_missing_tensors_and_workspaces_are_refused():
     g.d_table = base
     assert lib.vk_attend_backward(ctypes.byref(a), ctypes.byref(g), None, 0, None) == invalid and b"d_table" in lib.vk_last_error()
     g.d_table = None
+    assert lib.vk_attend_backward_workspace(ctypes.byref(a), ctypes.byref(size)) == vk.VK_OK and size.value > 0
+    assert lib.vk_attend_backward(ctypes.byref(a), ctypes.byref(g), None, 0, None) == invalid and b"workspace" in lib.vk_last_error()
+    assert lib.vk_attend_backward(ctypes.byref(a), ctypes.byref(g), base + 8, size.value, None) == invalid
     a.rows = base
     assert lib.vk_attend_backward(ctypes.byref(a), ctypes.byref(g), None, 0, None) == invalid and b"constants" in lib.vk_last_error()

@@ -189,16 +189,19 @@ def _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start) -> _A
     return _Attention.from_buffer(a)
 
 
-def _launch(call, size, device):
-    """Runs ``call(workspace, bytes, stream)`` on the device's current stream."""
+def _launch(entry, arguments, size, device):
+    """Calls ``entry(*arguments, workspace, bytes, stream)`` on the device's current stream."""
     work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     at = work.data_ptr() if size else None
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        _check(call(at, size, stream))
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = entry(*arguments, at, size, stream)
     else:
         with torch.cuda.device(device):
-            _check(call(at, size, stream))
+            rc = entry(*arguments, at, size, stream)
+    if rc:
+        _check(rc)
 
 
 def _forward(q, keys, values, rows, lengths, bias, q_start, scale, with_lse):
@@ -206,8 +209,7 @@ def _forward(q, keys, values, rows, lengths, bias, q_start, scale, with_lse):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(plan.lse_shape, dtype=torch.float32, device=q.device) if with_lse else None
     a = _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start)
-    vk_attend = library().vk_attend
-    _launch(lambda at, size, stream: vk_attend(a, at, size, stream), plan.forward_bytes, q.device)
+    _launch(library().vk_attend, (a,), plan.forward_bytes, q.device)
     return out, lse
 
 
@@ -286,6 +288,5 @@ def attend_backward(d_out: torch.Tensor, q: torch.Tensor, keys: torch.Tensor, va
     if bias is not None:
         d_table = like(bias.table)
         g.d_table = d_table.data_ptr()
-    vk_attend_backward = library().vk_attend_backward
-    _launch(lambda at, size, stream: vk_attend_backward(a, g, at, size, stream), plan.backward_bytes, q.device)
+    _launch(library().vk_attend_backward, (a, g), plan.backward_bytes, q.device)
     return Gradients(d_q, d_k, d_v, d_table)

@@ -13,7 +13,9 @@ constexpr int kMostDistance = 1024;  // largest max_distance: the bias by distan
 constexpr int kPad = 15;             // places at either end of the bias by distance (attend_tile.hpp)
 constexpr int kMostBiasBytes = 16384;  // biases by distance of the heads that share a block's columns; else a head alone
 constexpr int kKeyTile = 64;         // keys that a block of the tile kernels holds at once
+constexpr int kFewWaves = 8, kFewKeys = 32;  // waves of a block of the few-columns kernel, keys of its tiles
 constexpr int kFewPassages = 512;    // passages that a block of the few-columns kernel holds the rows of
+constexpr int grad_keys(int d) { return d <= 64 ? 64 : 32; }  // keys of a tile of the query gradient
 constexpr int kColumns = 128;        // query columns of a block of the tile kernels
 
 // A tensor [outer][middle][head][d]: element strides, d contiguous.
@@ -48,7 +50,7 @@ struct AttendArgs {
     // How the work is laid out. pack: query heads of one key head that share a block's columns (column = token * pack + head).
     // splits: runs of the keys that different blocks take, each of tiles_per_split places of passages x tiles.
     int pack = 1, splits = 1, tiles_per_split = 0;
-    float* part = nullptr;   // splits > 1: [splits][batch][heads / pack][tokens * pack][d] unnormalised sums ...
+    float* part = nullptr;   // splits > 1: [splits][batch][heads / pack][tokens * pack][d] unnormalised sums ... (d_q's parts alike)
     float2* stat = nullptr;  // ... and [splits][...][tokens * pack] (maximum, sum)
 };
 
@@ -57,7 +59,7 @@ struct AttendGradArgs {
     AttendView d_out, d_q, d_k, d_v;
     float scale = 0.f;            // the logits' own, which may be 0
     float* delta = nullptr;       // workspace [batch][heads][tokens]
-    float* table_part = nullptr;  // workspace [batch * column tiles][heads][buckets]
+    float* table_part = nullptr;  // workspace [splits * batch * column tiles][heads][buckets]
     void* d_table = nullptr;      // [buckets][heads], contiguous
 };
 
@@ -66,9 +68,10 @@ enum AttendType { kAttendF16 = 0, kAttendBf16 = 1 };
 hipError_t launch_attend_forward(const AttendArgs& a, int type, hipStream_t stream);
 hipError_t launch_attend_few(const AttendArgs& a, int type, hipStream_t stream);
 hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stream);
-// Writes d_q (and delta, and the table's partial sums).
+// Writes d_q, or its parts, delta and the table's partial sums.
 hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream);
 hipError_t launch_attend_grad_kv(const AttendGradArgs& g, int type, hipStream_t stream);
-hipError_t launch_attend_grad_table(const AttendGradArgs& g, int type, int parts, hipStream_t stream);
+// Joins what grad_q's splits wrote, and the table's partial sums.
+hipError_t launch_attend_grad_join(const AttendGradArgs& g, int type, int parts, hipStream_t stream);
 
 }  // namespace vk

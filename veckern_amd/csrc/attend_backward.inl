@@ -46,12 +46,6 @@ __device__ __forceinline__ void sum_diagonals(const float* skew, float* sums, in
     between_lanes();
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
-    return x;
-}
-
 // The first distance |x| of bucket j of a side.
 __device__ __forceinline__ int bucket_begin(const AttendBias& s, int j) {
     const int exact = s.side / 2;
@@ -61,7 +55,7 @@ __device__ __forceinline__ int bucket_begin(const AttendBias& s, int j) {
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     // with 128 elements a head two waves a SIMD have no registers for more
-    constexpr int kSteps = DP / 16, kParts = DP / 32, kKeys = DP == 64 ? 64 : 32, kSubs = kKeys / 32;
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kKeys = grad_keys(DP), kSubs = kKeys / 32;
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeys>];
     extern __shared__ float shared[];  // per wave a skewed tile; the bias by distance; per wave its gradient's sums by distance
@@ -71,6 +65,8 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     int place = xcd_place(blockIdx.x, gridDim.x);
     const int column_tile = place % column_tiles;
     place /= column_tiles;
+    const int split = place % a.splits;
+    place /= a.splits;
     const int group = place % groups, b = place / groups;
     const int kv_head = group * a.pack / (a.heads / a.kv_heads);
 
@@ -91,7 +87,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(x[j]), static_cast<float>(y[j]), delta);
     }
     delta = both_sum(delta);
-    if (used && hi == 0) g.delta[row] = delta;
+    if (used && hi == 0 && split == 0) g.delta[row] = delta;
     // rows without a key, and columns past the last: exp(x - inf) = 0
     float2 lse = used ? a.lse[row] : make_float2(-INFINITY, 0.f);
     lse = make_float2(lse.x == -INFINITY ? INFINITY : lse.x, lse.y * -kLog2e);
@@ -102,7 +98,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     for (int i = 0; i < kParts; ++i) dq[i] = f32x16{};
 
     KeyWalk<kKeys> walk;
-    walk.begin(a, b, 0, 0x7fffffff);
+    walk.begin(a, b, split * a.tiles_per_split, (split + 1) * a.tiles_per_split);
     Copier<DP, kKeys, 256> ks, vs;
     ks.init(thread, a.k.middle, a.d);
     vs.init(thread, a.v.middle, a.d);
@@ -235,7 +231,17 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     if (BIAS && large) run(std::integral_constant<bool, BIAS>());
     else run(std::false_type());
 
-    if (used) {
+    if (used && a.splits > 1) {
+        float* part = a.part + (((static_cast<int64_t>(split) * a.batch + b) * groups + group) * columns + c) * a.d;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const int e = 32 * i + mfma_row(4 * quad, hi);
+                if (e < a.d)
+                    *reinterpret_cast<f32x4*>(part + e) = f32x4{dq[i][4 * quad], dq[i][4 * quad + 1], dq[i][4 * quad + 2], dq[i][4 * quad + 3]};
+            }
+    } else if (used) {
         char* out = static_cast<char*>(g.d_q.p) + at(g.d_q) * 2;
 #pragma unroll
         for (int i = 0; i < kParts; ++i)
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             } else {
                 for (int y = max(from, 1); y < to; ++y) x += held[zero + y];
             }
-            g.table_part[((static_cast<int64_t>(b) * column_tiles + column_tile) * a.heads + head) * s.buckets + bucket] = x;
+            g.table_part[(((static_cast<int64_t>(split) * a.batch + b) * column_tiles + column_tile) * a.heads + head) * s.buckets + bucket] = x;
         }
     }
 }
@@ -669,7 +675,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
 template <class E, int DP>
 hipError_t launch_grad_q(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
-    const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns * (a.heads / a.pack) * a.batch;
+    const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns * (a.heads / a.pack) * a.batch * a.splits;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (4 * kSkewFloats + 5 * (2 * a.bias.far + 2 * kPad + 1)) * sizeof(float) : 0;
     auto kernel = a.bias.table ? grad_q_kernel<E, DP, true> : grad_q_kernel<E, DP, false>;

@@ -166,14 +166,36 @@ constexpr int64_t kUnits = 256;  // compute units of the card
 // Whether a call has so few columns for each key head that its time is the reading of the states.
 bool few_columns(const AttendArgs& a) { return static_cast<int64_t>(a.tokens) * a.pack <= 32; }
 
-// Splits the keys into runs of whole tiles until there are about `wanted` blocks, none with less than `least` tiles.
-void split_keys(AttendArgs& a, int tile, int64_t blocks, int64_t wanted, int least, int most_tiles) {
-    const int tiles = (a.length + tile - 1) / tile * a.passages;
-    int64_t splits = 1;
-    if (blocks > 0 && blocks < wanted) splits = std::min<int64_t>((wanted + blocks - 1) / blocks, tiles / least);
-    splits = std::max<int64_t>({splits, 1, (tiles + most_tiles - 1) / most_tiles});
-    a.tiles_per_split = static_cast<int>((tiles + splits - 1) / splits);
-    a.splits = a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
+// How long blocks of a kernel take, in microseconds as measured on this card: `start` for a block's first loads and its end,
+// `tile` for each of its tiles where a compute unit has one block, and `shared` of that more for each further block.
+struct Pace {
+    int resident;  // blocks that a compute unit holds at once
+    double start, tile, shared;
+};
+
+// Splits the keys into runs of whole tiles, for different blocks, where that makes a call shorter: the runs' parts are joined by
+// another launch (5 us) that reads what the runs wrote in 32 bits (3.5 TB/s). At the pace of the tile kernel one split of 256
+// blocks over 80 tiles of 64 elements a head took 107 us, two 75 + 6 and three, which fill the card, 63 + 7; of 18 blocks over 15
+// tiles of 128, one 26 us, five 12 + 4 and fifteen 12 + 7.
+void split_keys(AttendArgs& a, int tiles, int64_t blocks, const Pace& pace, int at_a_time, int most_tiles) {
+    const double part_bytes = 8.0 * a.batch * a.heads * a.tokens * a.d;
+    const int least = std::max(1, (tiles + most_tiles - 1) / std::max(most_tiles, 1));
+    double best = 0;
+    a.splits = 1;
+    a.tiles_per_split = tiles;
+    for (int s = least; s <= std::max(least, std::min(tiles, 64)); ++s) {
+        const int each = (tiles + s - 1) / s;
+        if (s > least && (tiles + each - 1) / each != s) continue;
+        const int64_t all = blocks * s, beside = std::max<int64_t>(1, std::min<int64_t>(pace.resident, (all + kUnits - 1) / kUnits));
+        const double rounds = static_cast<double>((all + kUnits * beside - 1) / (kUnits * beside));
+        const double time = rounds * (pace.start + (each + at_a_time - 1) / at_a_time * pace.tile * (1 + pace.shared * (beside - 1))) +
+                            (s > 1 ? 5 + s * part_bytes / 3.5e6 : 0);
+        if (s == least || time < best) {
+            best = time;
+            a.splits = each ? (tiles + each - 1) / each : 1;
+            a.tiles_per_split = each;
+        }
+    }
 }
 
 void plan_forward(AttendArgs& a) {
@@ -181,23 +203,36 @@ void plan_forward(AttendArgs& a) {
     a.pack = share;
     if (a.bias.table && static_cast<size_t>(share) * (2 * a.bias.far + 2 * vk::kPad + 1) * sizeof(float) > vk::kMostBiasBytes) a.pack = 1;
     const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
+    const bool small = a.d <= 64;
     if (few_columns(a)) {
-        const int per_row = (a.length + 31) / 32;  // a run of tiles touches one passage more than it fills
-        split_keys(a, 32, rest, kUnits, 32, std::max(1, (vk::kFewPassages - 1) * std::max(per_row, 1)));
+        const int per_row = (a.length + vk::kFewKeys - 1) / vk::kFewKeys;  // a run of tiles touches one passage more than it fills
+        split_keys(a, per_row * a.passages, rest, small ? Pace{2, 6.5, 0.8, 0.5} : Pace{1, 6.5, 2, 0}, vk::kFewWaves,
+                   (vk::kFewPassages - 1) * std::max(per_row, 1));
     } else {
-        split_keys(a, vk::kKeyTile, (columns + vk::kColumns - 1) / vk::kColumns * rest, 2 * kUnits, 1, 1 << 30);
+        split_keys(a, (a.length + vk::kKeyTile - 1) / vk::kKeyTile * a.passages, (columns + vk::kColumns - 1) / vk::kColumns * rest,
+                   small ? Pace{3, 6, 1.27, 0.34} : Pace{2, 6, 1.33, 0.66}, 1, 1 << 30);
     }
+}
+void plan_backward(AttendArgs& a) {
+    a.pack = a.bias.table ? 1 : a.heads / a.kv_heads;
+    const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
+    const int tile = vk::grad_keys(a.d);
+    split_keys(a, (a.length + tile - 1) / tile * a.passages, (columns + vk::kColumns - 1) / vk::kColumns * rest,
+               a.d <= 64 ? Pace{2, 10, 1.6, 0.5} : Pace{2, 10, 1.1, 0.5}, 1, 1 << 30);
 }
 size_t query_rows(const AttendArgs& a) { return static_cast<size_t>(a.batch) * a.heads * a.tokens; }
 size_t align(size_t x) { return (x + 15) / 16 * 16; }
 size_t forward_bytes(const AttendArgs& a) {
     return a.splits == 1 ? 0 : align(a.splits * query_rows(a) * a.d * sizeof(float)) + a.splits * query_rows(a) * sizeof(float2);
 }
-int table_parts(const AttendArgs& a) { return (a.tokens + vk::kColumns - 1) / vk::kColumns * a.batch; }
+int table_parts(const AttendArgs& a) { return (a.tokens + vk::kColumns - 1) / vk::kColumns * a.batch * a.splits; }
 size_t table_bytes(const AttendArgs& a) {
-    return a.bias.table ? static_cast<size_t>(table_parts(a)) * a.heads * a.bias.buckets * sizeof(float) : 0;
+    return a.bias.table ? align(static_cast<size_t>(table_parts(a)) * a.heads * a.bias.buckets * sizeof(float)) : 0;
 }
-size_t backward_bytes(const AttendArgs& a) { return align(query_rows(a) * sizeof(float)) + table_bytes(a); }
+size_t delta_bytes(const AttendArgs& a) { return align(query_rows(a) * sizeof(float)); }
+size_t backward_bytes(const AttendArgs& a) {
+    return delta_bytes(a) + table_bytes(a) + (a.splits == 1 ? 0 : a.splits * query_rows(a) * a.d * sizeof(float));
+}
 
 void check_workspace(void* workspace, size_t bytes, size_t needed) {
     valid(bytes >= needed && (workspace || !needed), "the workspace is too small");
@@ -250,7 +285,9 @@ VK_EXPORT int vk_attend(const vk_attention* x, void* workspace, size_t workspace
 VK_EXPORT int vk_attend_backward_workspace(const vk_attention* x, size_t* bytes) {
     return guarded([&] {
         valid(bytes != nullptr, "bytes is NULL");
-        *bytes = backward_bytes(args_of(x, false));
+        AttendArgs a = args_of(x, false);
+        plan_backward(a);
+        *bytes = backward_bytes(a);
     });
 }
 
@@ -275,13 +312,15 @@ VK_EXPORT int vk_attend_backward(const vk_attention* x, const vk_attention_grad*
         valid(a.bias.table || !y->d_table, "d_table is given without a table");
         g.d_table = y->d_table;
         g.scale = x->scale;
+        plan_backward(a);
         check_workspace(workspace, workspace_bytes, backward_bytes(a));
-        g.delta = static_cast<float*>(workspace);
-        g.table_part = reinterpret_cast<float*>(static_cast<char*>(workspace) + align(query_rows(a) * sizeof(float)));
-        a.pack = a.bias.table ? 1 : a.heads / a.kv_heads;
+        char* at = static_cast<char*>(workspace);
+        g.delta = reinterpret_cast<float*>(at);
+        g.table_part = reinterpret_cast<float*>(at + delta_bytes(a));
+        a.part = reinterpret_cast<float*>(at + delta_bytes(a) + table_bytes(a));
         const auto on = static_cast<hipStream_t>(stream);
         if (query_rows(a)) VK_HIP(vk::launch_attend_grad_q(g, x->type, on));
         if (!x->rows && x->bank && x->length) VK_HIP(vk::launch_attend_grad_kv(g, x->type, on));
-        if (a.bias.table) VK_HIP(vk::launch_attend_grad_table(g, x->type, table_parts(a), on));
+        if (a.bias.table || (a.splits > 1 && query_rows(a))) VK_HIP(vk::launch_attend_grad_join(g, x->type, table_parts(a), on));
     });
 }

@@ -9,8 +9,6 @@
 
 namespace vk::attend {
 
-constexpr int kFewWaves = 8, kFewKeys = 32;
-
 template <int DP>
 constexpr int kFewTiles = kFewWaves * 2 * kTileBytes<DP, kFewKeys>;
 static_assert(kFewWaves * 32 * (64 + 4) * 4 <= kFewTiles<64> && kFewWaves * 32 * (128 + 4) * 4 <= kFewTiles<128>,

@@ -1,5 +1,5 @@
-// What follows the attention kernels where their work was split: the joined softmax of the splits of a row, and the bias
-// table's gradient from the blocks' sums. Both sum in a fixed order.
+// What follows the attention kernels where their work was split: the joined softmax of the splits of a row, the query
+// gradient's parts, and the bias table's gradient from the blocks' sums. All sum in a fixed order.
 #include "attend_tile.hpp"
 
 namespace vk {
@@ -37,17 +37,36 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
     if (a.lse && e == 0) a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
 }
 
-// One wave per (bucket, head).
+// The first `query_blocks` blocks: d_q = scale * sum of the splits' parts, four elements a thread. The others: the table's
+// gradient, one wave per (bucket, head).
 template <class E>
-__global__ __launch_bounds__(256) void table_kernel(AttendGradArgs g, int parts) {
-    const int lane = threadIdx.x % 64, at = blockIdx.x * 4 + threadIdx.x / 64;
-    if (at >= g.a.heads * g.a.bias.buckets) return;
-    const int head = at % g.a.heads, bucket = at / g.a.heads;
+__global__ __launch_bounds__(256) void grad_join_kernel(AttendGradArgs g, int parts, int query_blocks) {
+    const AttendArgs& a = g.a;
+    if (static_cast<int>(blockIdx.x) < query_blocks) {
+        const int groups = a.heads / a.pack, columns = a.tokens * a.pack, quads = a.d / 4;
+        const int64_t rows = static_cast<int64_t>(a.batch) * groups * columns, at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+        if (at >= rows * quads) return;
+        const int64_t row = at / quads;
+        const int e = static_cast<int>(at - row * quads) * 4;
+        f32x4 x{};
+#pragma unroll 4
+        for (int i = 0; i < a.splits; ++i) x += *reinterpret_cast<const f32x4*>(a.part + (i * rows + row) * a.d + e);
+        const int c = row % columns, group = row / columns % groups, b = row / columns / groups;
+        const int token = c / a.pack, head = group * a.pack + c % a.pack;
+        typename E::T z[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[j] = (typename E::T)(x[j] * g.scale);
+        char* out = static_cast<char*>(g.d_q.p) + (b * g.d_q.outer + token * g.d_q.middle + head * g.d_q.head + e) * 2;
+        *reinterpret_cast<u32x2*>(out) = *reinterpret_cast<u32x2*>(z);
+        return;
+    }
+    const int lane = threadIdx.x % 64, at = (blockIdx.x - query_blocks) * 4 + threadIdx.x / 64;
+    if (at >= a.heads * a.bias.buckets) return;
+    const int head = at % a.heads, bucket = at / a.heads;
     float x = 0.f;
 #pragma unroll 4
-    for (int i = lane; i < parts; i += 64) x += g.table_part[(static_cast<int64_t>(i) * g.a.heads + head) * g.a.bias.buckets + bucket];
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
+    for (int i = lane; i < parts; i += 64) x += g.table_part[(static_cast<int64_t>(i) * a.heads + head) * a.bias.buckets + bucket];
+    x = wave_sum(x);
     if (lane == 0) static_cast<typename E::T*>(g.d_table)[at] = (typename E::T)x;
 }
 
@@ -61,9 +80,13 @@ hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stre
     return hipGetLastError();
 }
 
-hipError_t launch_attend_grad_table(const AttendGradArgs& g, int type, int parts, hipStream_t stream) {
-    auto kernel = type == kAttendBf16 ? attend::table_kernel<attend::Bf16> : attend::table_kernel<attend::F16>;
-    kernel<<<(g.a.heads * g.a.bias.buckets + 3) / 4, 256, 0, stream>>>(g, parts);
+hipError_t launch_attend_grad_join(const AttendGradArgs& g, int type, int parts, hipStream_t stream) {
+    const AttendArgs& a = g.a;
+    const int64_t queries = a.splits > 1 ? (static_cast<int64_t>(a.batch) * a.heads * a.tokens * (a.d / 4) + 255) / 256 : 0;
+    const int64_t blocks = queries + (a.bias.table ? (static_cast<int64_t>(a.heads) * a.bias.buckets + 3) / 4 : 0);
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    auto kernel = type == kAttendBf16 ? attend::grad_join_kernel<attend::Bf16> : attend::grad_join_kernel<attend::F16>;
+    kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(g, parts, static_cast<int>(queries));
     return hipGetLastError();
 }
 

@@ -58,6 +58,12 @@ __device__ __forceinline__ float both_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
+    return x;
+}
+
 // Tiles in LDS: rows of DP 16-bit elements, 16 bytes apart. A ds_read_b128 of 16 consecutive lanes takes 16 bytes of 16 rows,
 // the transposing read of 32 lanes 64 bytes of rows that are four apart: either covers the 64 banks of 4 bytes once. Every
 // place of a tile is one lane's address plus a constant, so the reads take two address registers in all.
