@@ -74,6 +74,13 @@ SHAPES = [
     (2, 128, 1, 128, 4, 4, 64, 0, False),
     (1, 129, 1, 257, 4, 1, 128, 0, False),
     (1, 300, 3, 70, 2, 1, 16, 0, True),
+    # many short passages: several in a tile, more than a block holds the rows of
+    (2, 40, 9, 17, 4, 2, 64, 0, True),
+    (3, 45, 30, 7, 2, 2, 128, 0, True),
+    (1, 3, 300, 5, 2, 1, 64, 40, True),
+    (1, 70, 600, 3, 2, 2, 128, 50, True),
+    (2, 1, 70, 33, 4, 1, 72, 40, True),
+    (1, 50, 280, 20, 1, 1, 32, 0, False),
 ]
 
 
@@ -89,7 +96,9 @@ def test_forward_and_gradients(shape, dtype):
 @pytest.mark.parametrize("kind", [(32, 128, True), (32, 128, False), (20, 100, False), (6, 9, True), (2, 2, False), (64, 512, True),
                                   (7, 40, False)], ids=str)
 @pytest.mark.parametrize("shape", [(2, 150, 1, 150, 3, 3, 64, 0, True), (2, 70, 2, 200, 4, 2, 80, 0, False),
-                                   (3, 5, 4, 131, 6, 2, 128, 11, True), (1, 1, 3, 40, 4, 4, 64, 5, False)], ids=str)
+                                   (3, 5, 4, 131, 6, 2, 128, 11, True), (1, 1, 3, 40, 4, 4, 64, 5, False),
+                                   (2, 60, 11, 21, 2, 1, 64, 0, True), (1, 33, 7, 50, 2, 2, 128, 0, True),
+                                   (1, 90, 5, 37, 2, 2, 64, 9, True)], ids=str)
 def test_position_bias(shape, kind, dtype):
     batch, tokens, passages, length, heads, kv_heads, d, bank, ragged = shape
     buckets, max_distance, two_sided = kind

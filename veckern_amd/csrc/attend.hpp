@@ -12,9 +12,10 @@ constexpr int kMostEdges = 128;      // bucket edges of a one-sided bias of 256 
 constexpr int kMostDistance = 1024;  // largest max_distance: the bias by distance, and its gradient, are held in LDS
 constexpr int kPad = 15;             // places at either end of the bias by distance (attend_tile.hpp)
 constexpr int kMostBiasBytes = 16384;  // biases by distance of the heads that share a block's columns; else a head alone
+constexpr int kSlot = 16;            // keys of a passage that stand together in a tile
 constexpr int kKeyTile = 64;         // keys that a block of the tile kernels holds at once
 constexpr int kFewWaves = 8, kFewKeys = 32;  // waves of a block of the few-columns kernel, keys of its tiles
-constexpr int kFewPassages = 512;    // passages that a block of the few-columns kernel holds the rows of
+constexpr int kHeldPassages = 256;   // passages that a block holds the rows of
 constexpr int grad_keys(int d) { return d <= 64 ? 64 : 32; }  // keys of a tile of the query gradient
 constexpr int kColumns = 128;        // query columns of a block of the tile kernels
 
@@ -48,7 +49,7 @@ struct AttendArgs {
     float scale = 0.f;            // positive, so that -inf * scale is -inf (0 is taken as 1e-37)
     AttendBias bias;
     // How the work is laid out. pack: query heads of one key head that share a block's columns (column = token * pack + head).
-    // splits: runs of the keys that different blocks take, each of tiles_per_split places of passages x tiles.
+    // splits: runs of the keys that different blocks take, each of tiles_per_split tiles.
     int pack = 1, splits = 1, tiles_per_split = 0;
     float* part = nullptr;   // splits > 1: [splits][batch][heads / pack][tokens * pack][d] unnormalised sums ... (d_q's parts alike)
     float2* stat = nullptr;  // ... and [splits][...][tokens * pack] (maximum, sum)

@@ -23,8 +23,7 @@ __device__ __forceinline__ void store_four(void* p, int at, const f32x16& x, int
 // Adds dS of a 32 x 32 tile (lane: one query position, x: the distance of the tile's first key from the first query) to a
 // wave's sums by distance, in a fixed order. The tile goes through LDS by diagonals: element (key, query) to row 31 + key -
 // query and place `query` of `skew`, whose other places stay zero; then a lane sums one diagonal and adds it to that distance's
-// place, or, beyond the far ends, to a register. With 36 floats a row neither the writes nor the 16-byte reads share a bank. The
-// two steps are apart so that products run between them. (Adding each element to its distance's place by an LDS atomic took 130
+// place, or, beyond the far ends, to a register. With 36 floats a row neither the writes nor the 16-byte reads share a bank. (Adding each element to its distance's place by an LDS atomic took 130
 // clocks an instruction.)
 constexpr int kSkew = 36, kSkewFloats = 63 * kSkew;
 __device__ __forceinline__ void put_diagonals(const f32x16& ds, float* skew, int lane) {
@@ -55,9 +54,10 @@ __device__ __forceinline__ int bucket_begin(const AttendBias& s, int j) {
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     // with 128 elements a head two waves a SIMD have no registers for more
-    constexpr int kSteps = DP / 16, kParts = DP / 32, kKeys = grad_keys(DP), kSubs = kKeys / 32;
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kKeys = grad_keys(DP), kSubs = kKeys / 32, kSlots = kKeys / kSlot;
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeys>];
+    __shared__ int2 found[kHeldPassages];
     extern __shared__ float shared[];  // per wave a skewed tile; the bias by distance; per wave its gradient's sums by distance
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
@@ -70,6 +70,8 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     const int group = place % groups, b = place / groups;
     const int kv_head = group * a.pack / (a.heads / a.kv_heads);
 
+    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
+    places.fill(a, b, found, thread, 256);
     const int c = column_tile * kColumns + wave * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
@@ -97,17 +99,16 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
 #pragma unroll
     for (int i = 0; i < kParts; ++i) dq[i] = f32x16{};
 
-    KeyWalk<kKeys> walk;
-    walk.begin(a, b, split * a.tiles_per_split, (split + 1) * a.tiles_per_split);
     Copier<DP, kKeys, 256> ks, vs;
     ks.init(thread, a.k.middle, a.d);
     vs.init(thread, a.v.middle, a.d);
+    __syncthreads();
+    KeyWalk<kSlots> walk(places, found);
     auto load = [&] {
-        const int valid = walk.count - walk.first;
-        ks.load(static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
-        vs.load(static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
+        ks.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
+        vs.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
     };
-    bool more = walk.valid();
+    bool more = walk.next();
     int now = 0;
     if (more) load();  // before the biases: what they wait for is under way with it
     int position = 0;
@@ -115,13 +116,13 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     bool large = false;
     float *held = nullptr, *sums = nullptr, *skew = nullptr;
     if constexpr (BIAS) {
-        const int places = bias_places(a.bias.far);
+        const int distances = bias_places(a.bias.far);
         skew = shared + wave * kSkewFloats;
         held = shared + 4 * kSkewFloats;
-        sums = held + (1 + wave) * places;
+        sums = held + (1 + wave) * distances;
         large = fill_biases<E>(a.bias, head, 1, a.scale, held, thread, 256);
         for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
-        for (int i = thread; i < 4 * places; i += 256) held[places + i] = 0.f;
+        for (int i = thread; i < 4 * distances; i += 256) held[distances + i] = 0.f;
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
 
@@ -155,10 +156,13 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     auto run = [&](auto kind) {
         constexpr bool kLarge = decltype(kind)::value;
         while (more) {
-            const int first = walk.first, left = walk.count - walk.first;
-            walk.next(a);
-            more = walk.valid();
+            Slot slots[kSlots];
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) slots[i] = walk.slots[i];
+            const bool full = walk.run || whole(slots);
+            more = walk.next();
             if (more) load();
+            const int2 at_keys = reach(slots);
             k = tile[now][0];
             v = tile[now][1];
             f32x16 s[kSubs] = {}, dp[kSubs] = {};
@@ -168,13 +172,14 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             if constexpr (BIAS) {
                 t0 = __builtin_amdgcn_readfirstlane(position);
                 if (!kLarge) {
-                    near = !far_apart(a.bias, first - (t0 + 31), first + kKeys - 1 - t0);
+                    near = !far_apart(a.bias, at_keys.x - (t0 + 31), at_keys.y - t0);
                     if (near) {
 #pragma unroll
                         for (int sub = 0; sub < kSubs; ++sub)
-                            each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position, [&](int r, float x) { s[sub][r] = x; });
+                            each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
+                                         [&](int r, float x) { s[sub][r] = x; });
                     } else {
-                        apart = held[bias_index(a.bias.far, first - position)] * a.scale;
+                        apart = held[bias_index(a.bias.far, at_keys.x - position)] * a.scale;
                     }
                 }
             }
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             if constexpr (kLarge) {
 #pragma unroll
                 for (int sub = 0; sub < kSubs; ++sub)
-                    each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position, [&](int r, float x) {
+                    each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position, [&](int r, float x) {
                         s[sub][r] = __builtin_fmaf(__builtin_fmaf(s[sub][r], a.scale, x) - lse.x, kLog2e, lse.y);
                     });
             } else {
@@ -195,31 +200,42 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             }
 #pragma unroll
             for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
-            if (left < kKeys) {
+            if (!full) {
 #pragma unroll
                 for (int r = 0; r < 16 * kSubs; ++r)
-                    if (r / 16 * 32 + tile_row(r % 16, hi) >= left) s[r / 16][r % 16] = 0.f;
+                    if (slot_row(r, hi) >= slots[r / 8].left) s[r / 16][r % 16] = 0.f;
             }
             if constexpr (BIAS) {
                 if (near) {
-                    put_diagonals(s[0], skew, lane);
+                    // a sub-tile whose two slots do not follow each other goes by each on its own
+#pragma unroll
+                    for (int sub = 0; sub < kSubs; ++sub) {
+                        const Slot &x = slots[2 * sub], &y = slots[2 * sub + 1];
+                        if (y.left && y.first != x.first + kSlot) {
+                            f32x16 one = s[sub];
+#pragma unroll
+                            for (int r = 0; r < 8; ++r) one[r] = 0.f;
+                            put_diagonals(one, skew, lane);
+                            sum_diagonals(skew, sums, a.bias.far, y.first - kSlot - t0, lane, below, above);
+                            one = s[sub];
+#pragma unroll
+                            for (int r = 8; r < 16; ++r) one[r] = 0.f;
+                            put_diagonals(one, skew, lane);
+                        } else {
+                            put_diagonals(s[sub], skew, lane);
+                        }
+                        sum_diagonals(skew, sums, a.bias.far, x.first - t0, lane, below, above);
+                    }
                 } else {
                     float all = 0.f;
 #pragma unroll
                     for (int r = 0; r < 16 * kSubs; ++r) all += s[r / 16][r % 16];
-                    if (first < position) below += all;
+                    if (at_keys.x < position) below += all;
                     else above += all;
                 }
             }
-            gather(s[0], 0);
 #pragma unroll
-            for (int sub = 1; sub <= kSubs; ++sub) {
-                if (BIAS && near) {
-                    sum_diagonals(skew, sums, a.bias.far, first + 32 * (sub - 1) - t0, lane, below, above);
-                    if (sub < kSubs) put_diagonals(s[sub], skew, lane);
-                }
-                if (sub < kSubs) gather(s[sub], sub);
-            }
+            for (int sub = 0; sub < kSubs; ++sub) gather(s[sub], sub);
             if (more) {
                 ks.store(tile[now ^ 1][0]);
                 vs.store(tile[now ^ 1][1]);
@@ -253,17 +269,17 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     }
     if constexpr (BIAS) {
         const AttendBias& s = a.bias;
-        const int places = bias_places(s.far), zero = s.far + kPad;  // the place of distance 0
+        const int distances = bias_places(s.far), zero = s.far + kPad;  // the place of distance 0
         below = wave_sum(below);
         above = wave_sum(above);
         if (lane == 0) {
             sums[0] += below;
-            sums[places - 1] += above;
+            sums[distances - 1] += above;
         }
         __syncthreads();
-        for (int i = thread; i < places; i += 256) {
+        for (int i = thread; i < distances; i += 256) {
             float x = 0.f;
-            for (int w = 1; w <= 4; ++w) x += held[w * places + i];
+            for (int w = 1; w <= 4; ++w) x += held[w * distances + i];
             held[i] = x;
         }
         __syncthreads();
@@ -282,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     }
 }
 
-// One block: 128 keys of a bank row and key head, each wave 32 of them; walks the request's query tiles, head by head.
+// One block: 128 keys of a request and key head (8 slots), each wave 32 of them; walks the request's query tiles, head by head.
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = 64;
@@ -294,21 +310,24 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
     extern __shared__ float bias_held[];
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
-    const int key_tiles = (a.length + kColumns - 1) / kColumns, share = a.heads / a.kv_heads;
+    const int share = a.heads / a.kv_heads, per_row = (a.length + kSlot - 1) / kSlot;
+    const int key_tiles = (per_row * a.passages + kColumns / kSlot - 1) / (kColumns / kSlot);
     int place = xcd_place(blockIdx.x, gridDim.x);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
-    const int kv_head = place % a.kv_heads;
-    const int row = place / a.kv_heads, b = row / a.passages;
-    const int count = row_length(a, row);
-    const int key = key_tile * kColumns + wave * 32 + lane % 32;
-    const bool there = key < count;
+    const int kv_head = place % a.kv_heads, b = place / a.kv_heads;
+    // the lane's key, by slots: of the passages of a request, 16 positions each
+    const int slot = key_tile * (kColumns / kSlot) + wave * 2 + lane % 32 / kSlot, passage = slot / per_row;
+    const int first_key = (slot - passage * per_row) * kSlot, key = first_key + lane % kSlot;
+    const bool inside = passage < a.passages;
+    const int row = b * a.passages + (inside ? passage : 0);
+    const bool there = inside && key < (a.lengths ? min(a.lengths[row], a.length) : a.length);
 
     f32x16 dk[kParts], dv[kParts];
 #pragma unroll
     for (int i = 0; i < kParts; ++i) dk[i] = dv[i] = f32x16{};
 
-    if (key_tile * kColumns < count) {
+    if (__syncthreads_or(there)) {
         s16x8 kf[kSteps], vf[kSteps];
         {
             const int64_t k = row * a.k.outer + key * a.k.middle + kv_head * a.k.head;
@@ -329,8 +348,8 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         int head = kv_head * share, first = 0;
         auto load = [&] {
             const int valid = a.tokens - first;
-            qs.load(static_cast<const char*>(a.q.p) + (b * a.q.outer + first * a.q.middle + head * a.q.head) * 2, valid);
-            ds.load(static_cast<const char*>(g.d_out.p) + (b * g.d_out.outer + first * g.d_out.middle + head * g.d_out.head) * 2, valid);
+            qs.load_rows(slot_start(a.q, {b, first, 0}, head), valid);
+            ds.load_rows(slot_start(g.d_out, {b, first, 0}, head), valid);
             if (thread < kQueries) {
                 const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + first + thread;
                 // nothing is computed from them before store(): that would wait for all loads under way
@@ -413,13 +432,13 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                 }
                 float apart = 0.f;  // a bias that all places of the tile share
                 if constexpr (BIAS && !kLarge) {
-                    const int k0 = key_tile * kColumns + wave * 32;
-                    if (far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start))) {
+                    const int x = __builtin_amdgcn_readfirstlane(first_key), y = __builtin_amdgcn_readlane(first_key, kSlot);
+                    if (far_apart(a.bias, min(x, y) - (from + kQueries - 1 + start), max(x, y) + kSlot - 1 - (from + start))) {
                         apart = bias_held[bias_index(a.bias.far, key - (from + start))] * scale_log2;
                     } else {
 #pragma unroll
                         for (int sub = 0; sub < 2; ++sub)
-                            each_bias<-1>(bias_held, a.bias.far, key - (from + start + 32 * sub + hi),
+                            each_bias<-1>(bias_held, a.bias.far, key - (from + start + 32 * sub + hi), key - (from + start + 32 * sub + 16 + hi),
                                           [&](int r, float x) { s[sub][r] += x; });
                     }
                 }
@@ -430,7 +449,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                 if constexpr (kLarge) {
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub) {
-                        each_bias<-1>(bias_held, a.bias.far, key - (from + start + 32 * sub + hi),
+                        each_bias<-1>(bias_held, a.bias.far, key - (from + start + 32 * sub + hi), key - (from + start + 32 * sub + 16 + hi),
                                       [&](int r, float x) { s[sub][r] = __builtin_fmaf(s[sub][r], a.scale, x); });
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
@@ -465,7 +484,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         else run(std::false_type());
     }
 
-    if (key < a.length) {  // keys past the row's length have no gradient: zeros
+    if (inside && key < a.length) {  // keys past the row's length have no gradient: zeros
         char* k = static_cast<char*>(g.d_k.p) + (row * g.d_k.outer + key * g.d_k.middle + kv_head * g.d_k.head) * 2;
         char* v = static_cast<char*>(g.d_v.p) + (row * g.d_v.outer + key * g.d_v.middle + kv_head * g.d_v.head) * 2;
 #pragma unroll
@@ -499,21 +518,24 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
 
     const int thread = threadIdx.x, lane = thread % 64, hi = lane / 32, wave = uniform(thread / 64) % 4;
     const bool second = uniform(thread / 256) != 0;
-    const int key_tiles = (a.length + kColumns - 1) / kColumns, share = a.heads / a.kv_heads;
+    const int share = a.heads / a.kv_heads, per_row = (a.length + kSlot - 1) / kSlot;
+    const int key_tiles = (per_row * a.passages + kColumns / kSlot - 1) / (kColumns / kSlot);
     int place = xcd_place(blockIdx.x, gridDim.x);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
-    const int kv_head = place % a.kv_heads;
-    const int row = place / a.kv_heads, b = row / a.passages;
-    const int count = row_length(a, row);
-    const int k0 = key_tile * kColumns + wave * 32, key = k0 + lane % 32;
-    const bool there = key < count;
+    const int kv_head = place % a.kv_heads, b = place / a.kv_heads;
+    // the lane's key, by slots: of the passages of a request, 16 positions each
+    const int slot = key_tile * (kColumns / kSlot) + wave * 2 + lane % 32 / kSlot, passage = slot / per_row;
+    const int first_key = (slot - passage * per_row) * kSlot, key = first_key + lane % kSlot;
+    const bool inside = passage < a.passages;
+    const int row = b * a.passages + (inside ? passage : 0);
+    const bool there = inside && key < (a.lengths ? min(a.lengths[row], a.length) : a.length);
 
     f32x16 sum[kParts];  // dV or dK
 #pragma unroll
     for (int i = 0; i < kParts; ++i) sum[i] = f32x16{};
 
-    if (key_tile * kColumns < count) {
+    if (__syncthreads_or(there)) {
         s16x8 own[kSteps];  // V or K
         {
             const AttendView& v = second ? a.v : a.k;
@@ -531,7 +553,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         float delta = 0.f;
         auto load = [&](int head, int first) {
             const int valid = a.tokens - first;
-            copier.load(static_cast<const char*>(rows.p) + (b * rows.outer + first * rows.middle + head * rows.head) * 2, valid);
+            copier.load_rows(slot_start(rows, {b, first, 0}, head), valid);
             if (thread < kQueries) {
                 const int64_t at = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + first + thread;
                 // nothing is computed from them before store(): that would wait for all loads under way
@@ -603,16 +625,17 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                     f32x16 s = kLarge ? f32x16{} : begin(now, 0);
                     float apart = 0.f;  // a bias that all places of the tile share
                     if constexpr (BIAS && !kLarge) {
-                        if (far_apart(a.bias, k0 - (from + kQueries - 1 + start), k0 + 31 - (from + start))) {
+                        const int x = __builtin_amdgcn_readfirstlane(first_key), y = __builtin_amdgcn_readlane(first_key, kSlot);
+                        if (far_apart(a.bias, min(x, y) - (from + kQueries - 1 + start), max(x, y) + kSlot - 1 - (from + start))) {
                             apart = bias_held[bias_index(a.bias.far, key - (from + start))] * scale_log2;
                         } else {
-                            each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), [&](int r, float x) { s[r] += x; });
+                            each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), key - (from + start + 16 + hi), [&](int r, float x) { s[r] += x; });
                         }
                     }
                     s = products(s, tile[now][0]);
                     if constexpr (kLarge) {
                         const f32x16 l = begin(now, 2), low = begin(now, 3);
-                        each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), [&](int r, float x) {
+                        each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), key - (from + start + 16 + hi), [&](int r, float x) {
                             s[r] = __builtin_fmaf(__builtin_fmaf(s[r], a.scale, x) - l[r], kLog2e, low[r]);
                         });
                     } else {
@@ -656,7 +679,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         else both(std::false_type());
     }
 
-    if (key < a.length) {  // keys past the row's length have no gradient: zeros
+    if (inside && key < a.length) {  // keys past the row's length have no gradient: zeros
         const AttendView& v = second ? g.d_k : g.d_v;
         char* out = static_cast<char*>(v.p) + (row * v.outer + key * v.middle + kv_head * v.head) * 2;
         const float factor = second ? g.scale : 1.f;
@@ -686,7 +709,8 @@ hipError_t launch_grad_q(const AttendGradArgs& g, hipStream_t stream) {
 template <class E, int DP>
 hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
-    const int64_t blocks = static_cast<int64_t>((a.length + kColumns - 1) / kColumns) * a.kv_heads * a.bank;
+    const int64_t slots = static_cast<int64_t>((a.length + kSlot - 1) / kSlot) * a.passages;
+    const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     if constexpr (DP == 64) {  // two waves for 32 keys: 170 us where one takes 142 (4 x 2048 tokens, 12 heads of 64)

@@ -109,7 +109,7 @@ AttendArgs args_of(const vk_attention* x, bool tensors) {
     valid(x->heads > 0 && x->kv_heads > 0 && x->heads % x->kv_heads == 0, "heads must be a multiple of kv_heads");
     valid(x->batch <= kMost && x->tokens <= kMost && x->passages <= kMost && x->length <= kMost && x->bank <= kMost && x->heads <= 65536,
           "a size is too large");
-    valid(x->tokens * x->heads <= kMost / 2 && (x->length + vk::kKeyTile) / vk::kKeyTile * x->passages <= kMost / 2 &&
+    valid(x->tokens * x->heads <= kMost / 2 && (x->length + vk::kSlot) / vk::kSlot * x->passages <= kMost / 16 &&
               x->length <= kMost / 2, "a size is too large");
     valid(std::isfinite(x->scale) && x->scale >= 0.f, "scale must be finite and not negative");
     valid(x->rows || x->bank == x->batch * x->passages, "without rows, bank must be batch * passages");
@@ -177,9 +177,13 @@ struct Pace {
 // another launch (5 us) that reads what the runs wrote in 32 bits (3.5 TB/s). At the pace of the tile kernel one split of 256
 // blocks over 80 tiles of 64 elements a head took 107 us, two 75 + 6 and three, which fill the card, 63 + 7; of 18 blocks over 15
 // tiles of 128, one 26 us, five 12 + 4 and fifteen 12 + 7.
-void split_keys(AttendArgs& a, int tiles, int64_t blocks, const Pace& pace, int at_a_time, int most_tiles) {
+void split_keys(AttendArgs& a, int keys, int64_t blocks, const Pace& pace, int at_a_time) {
     const double part_bytes = 8.0 * a.batch * a.heads * a.tokens * a.d;
-    const int least = std::max(1, (tiles + most_tiles - 1) / std::max(most_tiles, 1));
+    const int per_row = (a.length + vk::kSlot - 1) / vk::kSlot, per_tile = keys / vk::kSlot;
+    const int tiles = static_cast<int>((static_cast<int64_t>(per_row) * a.passages + per_tile - 1) / per_tile);
+    // a block holds the rows of kHeldPassages passages, and a run touches one more than it fills
+    const int64_t most_tiles = std::max<int64_t>(1, static_cast<int64_t>(vk::kHeldPassages - 1) * per_row / per_tile);
+    const int least = static_cast<int>(std::max<int64_t>(1, (tiles + most_tiles - 1) / most_tiles));
     double best = 0;
     a.splits = 1;
     a.tiles_per_split = tiles;
@@ -205,20 +209,17 @@ void plan_forward(AttendArgs& a) {
     const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
     const bool small = a.d <= 64;
     if (few_columns(a)) {
-        const int per_row = (a.length + vk::kFewKeys - 1) / vk::kFewKeys;  // a run of tiles touches one passage more than it fills
-        split_keys(a, per_row * a.passages, rest, small ? Pace{2, 6.5, 0.8, 0.5} : Pace{1, 6.5, 2, 0}, vk::kFewWaves,
-                   (vk::kFewPassages - 1) * std::max(per_row, 1));
+        split_keys(a, vk::kFewKeys, rest, small ? Pace{2, 6.5, 0.8, 0.5} : Pace{1, 6.5, 2, 0}, vk::kFewWaves);
     } else {
-        split_keys(a, (a.length + vk::kKeyTile - 1) / vk::kKeyTile * a.passages, (columns + vk::kColumns - 1) / vk::kColumns * rest,
-                   small ? Pace{3, 6, 1.27, 0.34} : Pace{2, 6, 1.33, 0.66}, 1, 1 << 30);
+        split_keys(a, vk::kKeyTile, (columns + vk::kColumns - 1) / vk::kColumns * rest,
+                   small ? Pace{3, 6, 1.27, 0.34} : Pace{2, 6, 1.33, 0.66}, 1);
     }
 }
 void plan_backward(AttendArgs& a) {
     a.pack = a.bias.table ? 1 : a.heads / a.kv_heads;
     const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
-    const int tile = vk::grad_keys(a.d);
-    split_keys(a, (a.length + tile - 1) / tile * a.passages, (columns + vk::kColumns - 1) / vk::kColumns * rest,
-               a.d <= 64 ? Pace{2, 10, 1.6, 0.5} : Pace{2, 10, 1.1, 0.5}, 1, 1 << 30);
+    split_keys(a, vk::grad_keys(a.d), (columns + vk::kColumns - 1) / vk::kColumns * rest,
+               a.d <= 64 ? Pace{2, 10, 1.6, 0.5} : Pace{2, 10, 1.1, 0.5}, 1);
 }
 size_t query_rows(const AttendArgs& a) { return static_cast<size_t>(a.batch) * a.heads * a.tokens; }
 size_t align(size_t x) { return (x + 15) / 16 * 16; }

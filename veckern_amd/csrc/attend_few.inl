@@ -16,7 +16,7 @@ static_assert(kFewWaves * 32 * (64 + 4) * 4 <= kFewTiles<64> && kFewWaves * 32 *
 
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(AttendArgs a) {
-    constexpr int kSteps = DP / 16, kParts = DP / 32, kThreads = 64 * kFewWaves;
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kThreads = 64 * kFewWaves, kSlots = kFewKeys / kSlot;
     extern __shared__ __align__(16) char shared[];  // tiles of each wave; (row, positions) of the passages; the bias by distance
     const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64), hi = lane / 32;
     const int columns = a.tokens * a.pack, column_tiles = (columns + 31) / 32, groups = a.heads / a.pack;
@@ -28,20 +28,10 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
     const int group = place % groups, b = place / groups;
     const int kv_head = group * a.pack / (a.heads / a.kv_heads);
 
-    const int per_row = (a.length + kFewKeys - 1) / kFewKeys;
-    const int begin = split * a.tiles_per_split, end = min(begin + a.tiles_per_split, per_row * a.passages);
+    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
     char* mine = shared + wave * 2 * kTileBytes<DP, kFewKeys>;
     int2* found = reinterpret_cast<int2*>(shared + kFewTiles<DP>);
-    const int r0 = per_row ? begin / per_row : 0;
-    if (begin < end) {
-        for (int r = r0 + thread; r <= (end - 1) / per_row; r += kThreads) {
-            int row = b * a.passages + r, count = a.length;
-            if (a.rows) row = a.rows[b * a.rows_outer + r * a.rows_step];
-            if (a.rows && (row < 0 || row >= a.bank)) count = 0;
-            else if (a.lengths) count = min(max(a.lengths[row], 0), a.length);
-            found[r - r0] = make_int2(row, count);
-        }
-    }
+    places.fill(a, b, found, thread, kThreads);
 
     const int c = column_tile * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
@@ -53,10 +43,10 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
     const float* held = nullptr;
     int position = 0;
     if constexpr (BIAS) {
-        float* all = reinterpret_cast<float*>(shared + kFewTiles<DP> + kFewPassages * sizeof(int2));
-        const int places = bias_places(a.bias.far);
-        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, 1.f, all + p * places, thread, kThreads);
-        held = all + (head - group * a.pack) * places;
+        float* all = reinterpret_cast<float*>(shared + kFewTiles<DP> + kHeldPassages * sizeof(int2));
+        const int distances = bias_places(a.bias.far);
+        for (int p = 0; p < a.pack; ++p) fill_bias<E>(a.bias, group * a.pack + p, 1.f, all + p * distances, thread, kThreads);
+        held = all + (head - group * a.pack) * distances;
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
     __syncthreads();
@@ -69,23 +59,32 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
     Copier<DP, kFewKeys, 64> ks, vs;
     ks.init(lane, a.k.middle, a.d);
     vs.init(lane, a.v.middle, a.d);
-    int at = begin + wave, r = at / max(per_row, 1), tile = at - r * per_row, first = 0, left = 0;
+    // the wave's next place, its passage and slot; the wave takes kSlots places of every kFewWaves * kSlots
+    int at = places.begin + wave * kSlots, r = places.per_row ? at / places.per_row : 0, step = at - r * places.per_row;
+    Slot slots[kSlots];
     // goes on to the wave's next tile with a key, and sets its loads going
     auto load = [&] {
-        for (; at < end; at += kFewWaves, tile += kFewWaves) {
-            while (tile >= per_row) {
-                tile -= per_row;
-                ++r;
+        while (at < places.end) {
+            int any = 0;
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) {
+                while (step >= places.per_row) {
+                    step -= places.per_row;
+                    ++r;
+                }
+                slots[i] = {0, 0, 0};
+                if (at + i < places.end) {
+                    const int2 x = found[r - places.r0];
+                    slots[i] = {uniform(x.x), step * kSlot, min(max(uniform(x.y) - step * kSlot, 0), kSlot)};
+                }
+                any += slots[i].left;
+                ++step;
             }
-            const int2 x = found[r - r0];
-            first = tile * kFewKeys;
-            left = uniform(x.y) - first;
-            if (left <= 0) continue;
-            const int64_t row = uniform(x.x);
-            ks.load(static_cast<const char*>(a.k.p) + (row * a.k.outer + first * a.k.middle + kv_head * a.k.head) * 2, left);
-            vs.load(static_cast<const char*>(a.v.p) + (row * a.v.outer + first * a.v.middle + kv_head * a.v.head) * 2, left);
-            at += kFewWaves;
-            tile += kFewWaves;
+            at += kFewWaves * kSlots;
+            step += (kFewWaves - 1) * kSlots;
+            if (!any) continue;
+            ks.load(slots, false, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
+            vs.load(slots, false, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
             return true;
         }
         return false;
@@ -95,22 +94,23 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
         ks.store(mine);
         vs.store(mine + kTileBytes<DP, kFewKeys>);
         between_lanes();
-        const int from = first, there = left;
+        const Slot here[kSlots] = {slots[0], slots[1]};
         more = load();
 
         f32x16 s{};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(mine, 0, i, lane), qf[i], s);
         if constexpr (BIAS) {
-            each_bias<1>(held, a.bias.far, from - position + hi, [&](int i, float x) { s[i] = __builtin_fmaf(s[i], a.scale, x); });
+            each_bias<1>(held, a.bias.far, here[0].first + hi - position, here[1].first + hi - position,
+                         [&](int i, float x) { s[i] = __builtin_fmaf(s[i], a.scale, x); });
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] *= a.scale;
         }
-        if (there < kFewKeys) {
+        if (!whole(here)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (tile_row(i, hi) >= there) s[i] = -INFINITY;
+                if (slot_row(i, hi) >= here[i / 8].left) s[i] = -INFINITY;
         }
         float most = s[0];
 #pragma unroll
@@ -159,8 +159,8 @@ __global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(A
         if (hi == 0) stats[wave * 32 + lane] = make_float2(top, total);
     }
     __syncthreads();
-    const int here = min(columns - column_tile * 32, 32), quads = a.d / 4;
-    for (int i = thread; i < here * quads; i += kThreads) {
+    const int held_columns = min(columns - column_tile * 32, 32), quads = a.d / 4;
+    for (int i = thread; i < held_columns * quads; i += kThreads) {
         const int x = i / quads, e = i % quads * 4;
         float most = -INFINITY, sum = 0.f;
         for (int w = 0; w < kFewWaves; ++w) most = fmaxf(most, stats[w * 32 + x].x);
@@ -193,7 +193,7 @@ template <class E, int DP>
 hipError_t launch_few(const AttendArgs& a, hipStream_t stream) {
     const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + 31) / 32 * a.splits * (a.heads / a.pack) * a.batch;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const size_t lds = kFewTiles<DP> + kFewPassages * sizeof(int2) +
+    const size_t lds = kFewTiles<DP> + kHeldPassages * sizeof(int2) +
                        (a.bias.table ? a.pack * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0);
     auto kernel = a.bias.table ? few_kernel<E, DP, true> : few_kernel<E, DP, false>;
     // more LDS than a kernel may have unasked; asked for once a device, for any bias
@@ -205,7 +205,7 @@ hipError_t launch_few(const AttendArgs& a, hipStream_t stream) {
     const uint64_t bit = uint64_t(1) << (device % 64);
     if (device >= 64 || !(done.load(std::memory_order_relaxed) & bit)) {
         e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                kFewTiles<DP> + static_cast<int>(kFewPassages * sizeof(int2)) + kMostBiasBytes);
+                                kFewTiles<DP> + static_cast<int>(kHeldPassages * sizeof(int2)) + kMostBiasBytes);
         if (e != hipSuccess) return e;
         done.fetch_or(bit, std::memory_order_relaxed);
     }

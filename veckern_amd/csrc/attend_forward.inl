@@ -17,8 +17,9 @@ namespace vk::attend {
 
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendArgs a) {
-    constexpr int kSteps = DP / 16, kParts = DP / 32;
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kSlots = kKeyTile / kSlot;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeyTile>];
+    __shared__ int2 found[kHeldPassages];
     extern __shared__ float bias_held[];
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
@@ -31,6 +32,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
     const int group = place % groups, b = place / groups;
     const int kv_head = group * a.pack / (a.heads / a.kv_heads);
 
+    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
+    places.fill(a, b, found, thread, 256);
     const int c = column_tile * kColumns + wave * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
@@ -44,17 +47,16 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
     for (int i = 0; i < kParts; ++i) o[i] = f32x16{};
     float top = -INFINITY, total = 0.f;
 
-    KeyWalk<kKeyTile> walk;
-    walk.begin(a, b, split * a.tiles_per_split, (split + 1) * a.tiles_per_split);
     Copier<DP, kKeyTile, 256> ks, vs;
     ks.init(thread, a.k.middle, a.d);
     vs.init(thread, a.v.middle, a.d);
+    __syncthreads();
+    KeyWalk<kSlots> walk(places, found);
     auto load = [&] {
-        const int valid = walk.count - walk.first;
-        ks.load(static_cast<const char*>(a.k.p) + (walk.row * a.k.outer + walk.first * a.k.middle + kv_head * a.k.head) * 2, valid);
-        vs.load(static_cast<const char*>(a.v.p) + (walk.row * a.v.outer + walk.first * a.v.middle + kv_head * a.v.head) * 2, valid);
+        ks.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
+        vs.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
     };
-    bool more = walk.valid();
+    bool more = walk.next();
     int now = 0;
     if (more) load();  // before the biases: what they wait for is under way with it
     const float* held = nullptr;
@@ -73,9 +75,11 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
     auto run = [&](auto kind) {
         constexpr bool kLarge = decltype(kind)::value;
         while (more) {
-            const int first = walk.first, left = walk.count - walk.first;
-            walk.next(a);
-            more = walk.valid();
+            Slot slots[kSlots];
+#pragma unroll
+            for (int i = 0; i < kSlots; ++i) slots[i] = walk.slots[i];
+            const bool full = walk.run || whole(slots);
+            more = walk.next();
             if (more) load();
 
             f32x16 s[2] = {};
@@ -83,12 +87,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
             if constexpr (BIAS && !kLarge) {
                 // the wave's tokens lie between its first and last column's
                 const int t0 = __builtin_amdgcn_readfirstlane(position), t1 = __builtin_amdgcn_readlane(position, 31);
-                if (far_apart(a.bias, first - t1, first + kKeyTile - 1 - t0)) {
-                    apart = held[bias_index(a.bias.far, first - position)] * a.scale;
+                const int2 at = reach(slots);
+                if (far_apart(a.bias, at.x - t1, at.y - t0)) {
+                    apart = held[bias_index(a.bias.far, at.x - position)] * a.scale;
                 } else {
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub)
-                        each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position, [&](int r, float x) { s[sub][r] = x; });
+                        each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
+                                     [&](int r, float x) { s[sub][r] = x; });
                 }
             }
             __builtin_amdgcn_s_setprio(1);
@@ -103,13 +109,13 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendAr
             if constexpr (kLarge) {
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub)
-                    each_bias<1>(held, a.bias.far, first + 32 * sub + hi - position,
+                    each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
                                  [&](int r, float x) { s[sub][r] = __builtin_fmaf(s[sub][r], a.scale, x); });
             }
-            if (left < kKeyTile) {
+            if (!full) {
 #pragma unroll
                 for (int r = 0; r < 32; ++r)
-                    if (r / 16 * 32 + tile_row(r % 16, hi) >= left) s[r / 16][r % 16] = -INFINITY;
+                    if (slot_row(r, hi) >= slots[r / 8].left) s[r / 16][r % 16] = -INFINITY;
             }
             float most = s[0][0];
 #pragma unroll

@@ -72,28 +72,58 @@ constexpr int kPitch = DP * 2 + 16;
 template <int DP, int ROWS>
 constexpr int kTileBytes = ROWS * kPitch<DP>;
 
-// Copies ROWS rows of a tensor into such a tile through registers; rows past `valid` and elements past d become zero (the
-// buffer descriptor's range check), so nothing of what lies there, infinities and NaN included, reaches a product.
+// A tile's rows come in slots of 16: `left` positions from `first` on of a bank row, so that short passages share a tile.
+struct Slot {
+    int row, first, left;
+};
+__device__ __forceinline__ int slot_row(int r, int hi) { return tile_row(r % 8, hi); }  // of the slot that result r belongs to
+
+// Copies ROWS rows of a tensor into such a tile through registers; rows past a slot's and elements past d become zero (the
+// buffer descriptor's range check), so nothing of what lies there, infinities and NaN included, reaches a product. The rows that
+// a wave copies in one step are of one slot.
 template <int DP, int ROWS, int THREADS>
 struct Copier {
-    static constexpr int kChunks = DP / 8, kEach = ROWS * kChunks / THREADS, kRows = THREADS / kChunks;
+    static constexpr int kChunks = DP / 8, kEach = ROWS * kChunks / THREADS, kRows = THREADS / kChunks, kWaveRows = 64 / kChunks;
     static_assert(ROWS * kChunks % THREADS == 0 && THREADS % kChunks == 0, "every thread copies the same chunk of some rows");
+    static_assert(kSlot % kWaveRows == 0 && (kRows % kSlot == 0 || kSlot % kRows == 0), "a wave's rows of a step are of one slot");
     static constexpr int kOut = int(0x80000000u);  // past every descriptor's range
-    int row, offset, step, to;
+    int row, offset, step, to, wave_row;
     u32x4 held[kEach];
 
     __device__ void init(int thread, int64_t stride, int d) {
-        row = thread / kChunks;
         const int chunk = thread % kChunks;
+        row = thread / kChunks % kSlot;
+        wave_row = __builtin_amdgcn_readfirstlane(thread / 64) * kWaveRows;
         offset = chunk * 8 < d ? static_cast<int>(row * stride * 2) + chunk * 16 : kOut;
-        step = static_cast<int>(kRows * stride * 2);
-        to = row * kPitch<DP> + chunk * 16;
+        step = static_cast<int>(stride * 2);
+        to = thread / kChunks * kPitch<DP> + chunk * 16;
     }
-    __device__ void load(const void* base, int valid) {
-        auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+    // base(slot): where the slot's first row starts; run: the slots are full and follow each other in one row
+    template <class F>
+    __device__ void load(const Slot (&slots)[ROWS / kSlot], bool run, F&& base) {
+        if (run) return load_rows(base(slots[0]), ROWS);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            held[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row + kRows * i < valid ? offset + step * i : kOut, 0, 0);
+        for (int i = 0; i < kEach; ++i) {
+            const int at = wave_row + kRows * i, skipped = kRows * i % kSlot;
+            Slot s = slots[kRows * i / kSlot];
+            if constexpr (kRows > kSlot) {  // the waves of a step copy different slots
+#pragma unroll
+                for (int j = kRows * i / kSlot + 1; j < kRows * (i + 1) / kSlot; ++j)
+                    if (at / kSlot == j) s = slots[j];
+            }
+            auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base(s)), 0, 0x7fffffff, 0x00020000);
+            held[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row + skipped < s.left ? offset + step * skipped : kOut, 0, 0);
+        }
+    }
+    // The first `valid` of ROWS rows that follow each other.
+    __device__ void load_rows(const char* base, int valid) {
+        auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, 0x7fffffff, 0x00020000);
+        const int skipped = kRows > kSlot ? wave_row / kSlot * kSlot : 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int rows = kRows * i + skipped;
+            held[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row + rows < valid ? offset + step * rows : kOut, 0, 0);
+        }
     }
     __device__ void store(char* tile) const {
 #pragma unroll
@@ -151,54 +181,94 @@ __device__ __forceinline__ float2 logarithm(float top, float total) {
 // One scalar-register value from a load whose address is the same in all lanes.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The bank row of passage r of request b, or -1 where there is none; rows outside the bank count as none.
-__device__ __forceinline__ int64_t bank_row(const AttendArgs& a, int b, int r) {
-    if (!a.rows) return static_cast<int64_t>(b) * a.passages + r;
-    const int id = uniform(a.rows[b * a.rows_outer + r * a.rows_step]);
-    return id >= 0 && id < a.bank ? id : -1;
+// The bank row of passage r of request b and how many positions it holds: none for a row outside the bank.
+__device__ __forceinline__ int2 find_row(const AttendArgs& a, int b, int r) {
+    int row = b * a.passages + r, count = a.length;
+    if (a.rows) row = a.rows[b * a.rows_outer + r * a.rows_step];
+    if (a.rows && (row < 0 || row >= a.bank)) return make_int2(0, 0);
+    if (a.lengths) count = min(max(a.lengths[row], 0), a.length);
+    return make_int2(row, count);
 }
-__device__ __forceinline__ int row_length(const AttendArgs& a, int64_t row) {
-    if (row < 0) return 0;
-    if (!a.lengths) return a.length;
-    return min(max(uniform(a.lengths[row]), 0), a.length);
-}
-
-// Walks the tiles of KEYS keys that have at least one (of `row`, from `first` on; the row holds `count`), of the places
-// [begin, end) of passages x tiles.
-template <int KEYS>
-struct KeyWalk {
-    int b, r, per_row, end, first, count;
-    int64_t row;
-
-    __device__ void begin(const AttendArgs& a, int batch, int place, int last) {
-        b = batch;
-        per_row = (a.length + KEYS - 1) / KEYS;
-        end = min(last, per_row * a.passages);
-        r = place / max(per_row, 1);
-        first = (place - r * per_row) * KEYS;
-        if (place < end) {
-            row = bank_row(a, b, r);
-            count = row_length(a, row);
-            settle(a);
-        } else {
-            r = a.passages;
-        }
+// A request's keys are counted in places: slots of its passages, empty ones included, passage by passage. A block holds the rows
+// of the passages that its places [begin, end) lie in.
+struct Places {
+    int per_row, begin, end, r0;
+    __device__ Places(const AttendArgs& a, int from, int count) {
+        per_row = (a.length + kSlot - 1) / kSlot;
+        begin = from;
+        end = min(from + count, per_row * a.passages);
+        r0 = begin < end ? begin / per_row : 0;
     }
-    __device__ bool valid() const { return r * per_row + first / KEYS < end; }
-    __device__ void next(const AttendArgs& a) {
-        first += KEYS;
-        settle(a);
-    }
-    __device__ void settle(const AttendArgs& a) {
-        while (first >= count) {
-            ++r;
-            first = 0;
-            if (r * per_row >= end) return;
-            row = bank_row(a, b, r);
-            count = row_length(a, row);
-        }
+    __device__ void fill(const AttendArgs& a, int b, int2* found, int thread, int threads) const {
+        if (begin < end)
+            for (int r = r0 + thread; r <= (end - 1) / per_row; r += threads) found[r - r0] = find_row(a, b, r);
     }
 };
+
+// Walks the slots that hold a key, SLOTS at a time.
+template <int SLOTS>
+struct KeyWalk {
+    Slot slots[SLOTS];
+    bool run;  // the slots are full and follow each other in one row
+    const int2* found;
+    int per_row, end, r0, r, step, row, count;
+
+    __device__ KeyWalk(const Places& p, const int2* held) : found(held), per_row(p.per_row), end(p.end), r0(p.r0), r(p.r0) {
+        step = p.begin - p.r0 * per_row;
+        row = count = 0;
+        if (p.begin < end) take();
+        else r = end;
+    }
+    __device__ void take() {
+        row = uniform(found[r - r0].x);
+        count = uniform(found[r - r0].y);
+    }
+    // The next tile's slots, empty ones at the end; false where none is left.
+    __device__ bool next() {
+        const int first = step * kSlot;
+        run = count - first >= SLOTS * kSlot && r * per_row + step + SLOTS <= end;
+        if (run) {
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) slots[i] = {row, first + kSlot * i, kSlot};
+            step += SLOTS;
+            return true;
+        }
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            slots[i] = {0, 0, 0};
+            while (r * per_row + step < end) {
+                if (step * kSlot < count) {
+                    slots[i] = {row, step * kSlot, min(count - step * kSlot, kSlot)};
+                    ++step;
+                    break;
+                }
+                step = count = 0;
+                if (++r * per_row < end) take();
+            }
+        }
+        return slots[0].left > 0;
+    }
+};
+// Where a slot's first position starts, of a key head.
+__device__ __forceinline__ const char* slot_start(const AttendView& v, const Slot& s, int head) {
+    return static_cast<const char*>(v.p) + (s.row * v.outer + s.first * v.middle + head * v.head) * 2;
+}
+// Whether all of a tile's places hold a key, and the first and last position of any.
+template <int SLOTS>
+__device__ __forceinline__ bool whole(const Slot (&s)[SLOTS]) {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) all = all && s[i].left == kSlot;
+    return all;
+}
+template <int SLOTS>
+__device__ __forceinline__ int2 reach(const Slot (&s)[SLOTS]) {
+    int2 x = make_int2(s[0].first, s[0].first);
+#pragma unroll
+    for (int i = 1; i < SLOTS; ++i)
+        if (s[i].left) x = make_int2(min(x.x, s[i].first), max(x.y, s[i].first));
+    return make_int2(x.x, x.y + kSlot - 1);
+}
 
 // Blocks that read the same keys follow each other in the order of `place`; the hardware deals block ids over the 8 XCDs in
 // turn, so each XCD is given one run of places and its L2 sees the same keys again.
@@ -266,12 +336,13 @@ __device__ __forceinline__ bool far_apart(const AttendBias& s, int least, int mo
     return most <= -s.far || least >= (s.two_sided ? s.far : 0);
 }
 
-// The biases of a 32 x 32 tile. x0: the distance at tile_row(0, hi) of the lane; STEP: how it changes from row to row.
+// The biases at 16 of a lane's results, 8 for each of two slots. x0, x1: the distances at their tile_row(0, hi); STEP: how a
+// distance changes from row to row.
 template <int STEP, class F>
-__device__ __forceinline__ void each_bias(const float* held, int far, int x0, F&& use) {
+__device__ __forceinline__ void each_bias(const float* held, int far, int x0, int x1, F&& use) {
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
-        const int x = x0 + STEP * 16 * part;
+        const int x = part ? x1 : x0;
         const float* at = held + bias_index(far, STEP > 0 ? x : x - 14);
 #pragma unroll
         for (int r = 0; r < 8; ++r) use(8 * part + r, at[STEP > 0 ? tile_row(r, 0) : 14 - tile_row(r, 0)]);
