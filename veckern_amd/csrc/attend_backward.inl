@@ -713,7 +713,7 @@ hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
-    if constexpr (DP == 64) {  // two waves for 32 keys: 170 us where one takes 142 (4 x 2048 tokens, 12 heads of 64)
+    if constexpr (DP <= 64) {  // two waves for 32 keys: 170 us where one takes 142 (4 x 2048 tokens, 12 heads of 64)
         auto kernel = a.bias.table ? grad_kv_kernel<E, DP, true> : grad_kv_kernel<E, DP, false>;
         kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
     } else {  // one wave for 32 keys: 767 us where two take 603 (2 x 2048 tokens over 4 x 2048 keys, 16 heads of 128)

@@ -1,0 +1,7 @@
+// Backward tile kernels for bf16 inputs and head sizes up to 32.
+#include "attend_backward.inl"
+
+namespace vk {
+hipError_t attend_grad_q_bf16_32(const AttendGradArgs& g, hipStream_t stream) { return attend::launch_grad_q<attend::Bf16, 32>(g, stream); }
+hipError_t attend_grad_kv_bf16_32(const AttendGradArgs& g, hipStream_t stream) { return attend::launch_grad_kv<attend::Bf16, 32>(g, stream); }
+}  // namespace vk

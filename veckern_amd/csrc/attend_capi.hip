@@ -13,26 +13,31 @@ namespace vk {
     hipError_t attend_few_##type##_##size(const AttendArgs& a, hipStream_t stream);         \
     hipError_t attend_grad_q_##type##_##size(const AttendGradArgs& g, hipStream_t stream);  \
     hipError_t attend_grad_kv_##type##_##size(const AttendGradArgs& g, hipStream_t stream);
+VK_ATTEND_INSTANCES(bf16, 32)
 VK_ATTEND_INSTANCES(bf16, 64)
+VK_ATTEND_INSTANCES(bf16, 96)
 VK_ATTEND_INSTANCES(bf16, 128)
+VK_ATTEND_INSTANCES(f16, 32)
 VK_ATTEND_INSTANCES(f16, 64)
+VK_ATTEND_INSTANCES(f16, 96)
 VK_ATTEND_INSTANCES(f16, 128)
 
+// The instance of the type and of the next of 32, 64, 96 and 128 elements a head.
+#define VK_ATTEND_PICK(name, type, d)                                                                                     \
+    ((type) == kAttendBf16 ? ((d) <= 32 ? name##_bf16_32 : (d) <= 64 ? name##_bf16_64 : (d) <= 96 ? name##_bf16_96 : name##_bf16_128) \
+                           : ((d) <= 32 ? name##_f16_32 : (d) <= 64 ? name##_f16_64 : (d) <= 96 ? name##_f16_96 : name##_f16_128))
+
 hipError_t launch_attend_forward(const AttendArgs& a, int type, hipStream_t stream) {
-    if (type == kAttendBf16) return a.d <= 64 ? attend_forward_bf16_64(a, stream) : attend_forward_bf16_128(a, stream);
-    return a.d <= 64 ? attend_forward_f16_64(a, stream) : attend_forward_f16_128(a, stream);
+    return VK_ATTEND_PICK(attend_forward, type, a.d)(a, stream);
 }
 hipError_t launch_attend_few(const AttendArgs& a, int type, hipStream_t stream) {
-    if (type == kAttendBf16) return a.d <= 64 ? attend_few_bf16_64(a, stream) : attend_few_bf16_128(a, stream);
-    return a.d <= 64 ? attend_few_f16_64(a, stream) : attend_few_f16_128(a, stream);
+    return VK_ATTEND_PICK(attend_few, type, a.d)(a, stream);
 }
 hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream) {
-    if (type == kAttendBf16) return g.a.d <= 64 ? attend_grad_q_bf16_64(g, stream) : attend_grad_q_bf16_128(g, stream);
-    return g.a.d <= 64 ? attend_grad_q_f16_64(g, stream) : attend_grad_q_f16_128(g, stream);
+    return VK_ATTEND_PICK(attend_grad_q, type, g.a.d)(g, stream);
 }
 hipError_t launch_attend_grad_kv(const AttendGradArgs& g, int type, hipStream_t stream) {
-    if (type == kAttendBf16) return g.a.d <= 64 ? attend_grad_kv_bf16_64(g, stream) : attend_grad_kv_bf16_128(g, stream);
-    return g.a.d <= 64 ? attend_grad_kv_f16_64(g, stream) : attend_grad_kv_f16_128(g, stream);
+    return VK_ATTEND_PICK(attend_grad_kv, type, g.a.d)(g, stream);
 }
 
 }  // namespace vk

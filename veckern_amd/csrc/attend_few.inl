@@ -11,11 +11,12 @@ namespace vk::attend {
 
 template <int DP>
 constexpr int kFewTiles = kFewWaves * 2 * kTileBytes<DP, kFewKeys>;
-static_assert(kFewWaves * 32 * (64 + 4) * 4 <= kFewTiles<64> && kFewWaves * 32 * (128 + 4) * 4 <= kFewTiles<128>,
-              "the waves' outputs are joined where the tiles were");
+template <int DP>
+constexpr bool kJoinFits = kFewWaves * 32 * (DP + 4) * 4 <= kFewTiles<DP>;
+static_assert(kJoinFits<32> && kJoinFits<64> && kJoinFits<96> && kJoinFits<128>, "the waves' outputs are joined where the tiles were");
 
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(64 * kFewWaves, DP == 64 ? 4 : 2) void few_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(AttendArgs a) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kThreads = 64 * kFewWaves, kSlots = kFewKeys / kSlot;
     extern __shared__ __align__(16) char shared[];  // tiles of each wave; (row, positions) of the passages; the bias by distance
     const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64), hi = lane / 32;

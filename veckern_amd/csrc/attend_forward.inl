@@ -16,7 +16,7 @@
 namespace vk::attend {
 
 template <class E, int DP, bool BIAS>
-__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void forward_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendArgs a) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kSlots = kKeyTile / kSlot;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeyTile>];
     __shared__ int2 found[kHeldPassages];

@@ -1,0 +1,6 @@
+// Forward tile kernels for bf16 inputs and head sizes up to 96.
+#include "attend_forward.inl"
+
+namespace vk {
+hipError_t attend_forward_bf16_96(const AttendArgs& a, hipStream_t stream) { return attend::launch_forward<attend::Bf16, 96>(a, stream); }
+}  // namespace vk

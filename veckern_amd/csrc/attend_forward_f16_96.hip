@@ -1,0 +1,6 @@
+// Forward tile kernels for f16 inputs and head sizes up to 96.
+#include "attend_forward.inl"
+
+namespace vk {
+hipError_t attend_forward_f16_96(const AttendArgs& a, hipStream_t stream) { return attend::launch_forward<attend::F16, 96>(a, stream); }
+}  // namespace vk

@@ -83,15 +83,19 @@ __device__ __forceinline__ int slot_row(int r, int hi) { return tile_row(r % 8, 
 // a wave copies in one step are of one slot.
 template <int DP, int ROWS, int THREADS>
 struct Copier {
-    static constexpr int kChunks = DP / 8, kEach = ROWS * kChunks / THREADS, kRows = THREADS / kChunks, kWaveRows = 64 / kChunks;
+    // threads to a row: as many as it has chunks, or, for 96 elements, four that only keep the rows apart
+    static constexpr int kChunks = DP == 96 ? 16 : DP / 8;
+    static constexpr int kEach = ROWS * kChunks / THREADS, kRows = THREADS / kChunks, kWaveRows = 64 / kChunks;
     static_assert(ROWS * kChunks % THREADS == 0 && THREADS % kChunks == 0, "every thread copies the same chunk of some rows");
     static_assert(kSlot % kWaveRows == 0 && (kRows % kSlot == 0 || kSlot % kRows == 0), "a wave's rows of a step are of one slot");
     static constexpr int kOut = int(0x80000000u);  // past every descriptor's range
     int row, offset, step, to, wave_row;
+    bool mine;
     u32x4 held[kEach];
 
     __device__ void init(int thread, int64_t stride, int d) {
         const int chunk = thread % kChunks;
+        mine = chunk < DP / 8;
         row = thread / kChunks % kSlot;
         wave_row = __builtin_amdgcn_readfirstlane(thread / 64) * kWaveRows;
         offset = chunk * 8 < d ? static_cast<int>(row * stride * 2) + chunk * 16 : kOut;
@@ -127,7 +131,8 @@ struct Copier {
     }
     __device__ void store(char* tile) const {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) *reinterpret_cast<u32x4*>(tile + to + kRows * i * kPitch<DP>) = held[i];
+        for (int i = 0; i < kEach; ++i)
+            if (DP != 96 || mine) *reinterpret_cast<u32x4*>(tile + to + kRows * i * kPitch<DP>) = held[i];
     }
 };
 
@@ -350,10 +355,11 @@ __device__ __forceinline__ void each_bias(const float* held, int far, int x0, in
 }
 
 // Instruction order of a run of `n` products of the matrix cores whose first operands come from LDS, `reads` reads each: the
-// reads are kept `ahead` products in front, as a read takes about as long as three to four products, and `others` vector
+// reads are kept `most` products in front, as a read takes about as long as three to four products, and `others` vector
 // instructions of another part of the tile, that runs beside it, follow each product.
-template <int n, int reads, int ahead, int others = 0>
+template <int n, int reads, int most, int others = 0>
 __device__ __forceinline__ void feed() {
+    constexpr int ahead = most < n ? most : n;
     __builtin_amdgcn_sched_group_barrier(0x100, reads * ahead, 0);
 #pragma unroll
     for (int i = 0; i < n; ++i) {
