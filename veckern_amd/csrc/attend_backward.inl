@@ -70,31 +70,22 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     const int group = place % groups, b = place / groups;
     const int kv_head = group * a.pack / (a.heads / a.kv_heads);
 
-    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
-    places.fill(a, b, found, thread, 256);
     const int c = column_tile * kColumns + wave * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
     const int64_t row = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + token;
     auto at = [&](const AttendView& v) { return b * v.outer + token * v.middle + head * v.head; };
-    s16x8 qf[kSteps], df[kSteps];
-    float delta = 0.f;
+    s16x8 qf[kSteps], df[kSteps], of[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
         qf[i] = column(a.q, at(a.q), used, i, hi, a.d);
         df[i] = column(g.d_out, at(g.d_out), used, i, hi, a.d);
-        const auto x = __builtin_bit_cast(typename E::x8, df[i]);
-        const auto y = __builtin_bit_cast(typename E::x8, column(a.out, at(a.out), used, i, hi, a.d));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(x[j]), static_cast<float>(y[j]), delta);
+        of[i] = column(a.out, at(a.out), used, i, hi, a.d);
     }
-    delta = both_sum(delta);
-    if (used && hi == 0 && split == 0) g.delta[row] = delta;
-    // rows without a key, and columns past the last: exp(x - inf) = 0
     float2 lse = used ? a.lse[row] : make_float2(-INFINITY, 0.f);
-    lse = make_float2(lse.x == -INFINITY ? INFINITY : lse.x, lse.y * -kLog2e);
+    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
+    places.fill(a, b, found, thread, 256);
 
-    const float scale_log2 = a.scale * kLog2e;
     f32x16 dq[kParts];
 #pragma unroll
     for (int i = 0; i < kParts; ++i) dq[i] = f32x16{};
@@ -126,6 +117,18 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
 
+    float delta = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const auto x = __builtin_bit_cast(typename E::x8, df[i]), y = __builtin_bit_cast(typename E::x8, of[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(x[j]), static_cast<float>(y[j]), delta);
+    }
+    delta = both_sum(delta);
+    if (used && hi == 0 && split == 0) g.delta[row] = delta;
+    // rows without a key, and columns past the last: exp(x - inf) = 0
+    lse = make_float2(lse.x == -INFINITY ? INFINITY : lse.x, lse.y * -kLog2e);
+    const float scale_log2 = a.scale * kLog2e;
     if (more) {
         ks.store(tile[0][0]);
         vs.store(tile[0][1]);
@@ -283,17 +286,20 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             held[i] = x;
         }
         __syncthreads();
-        for (int bucket = thread; bucket < s.buckets; bucket += 256) {
+        for (int bucket = thread / 8; bucket < (s.buckets + 31) / 32 * 32; bucket += 32) {  // eight lanes each
             const int j = bucket % s.side, from = bucket_begin(s, j), to = j + 1 < s.side ? bucket_begin(s, j + 1) : zero + 1;
             float x = 0.f;
             if (bucket < s.side) {
-                for (int y = from; y < to; ++y) x += held[zero - y];
+                for (int y = from + thread % 8; y < to; y += 8) x += held[zero - y];
                 if (!s.two_sided && j == 0)
-                    for (int y = 1; y <= zero; ++y) x += held[zero + y];
-            } else {
-                for (int y = max(from, 1); y < to; ++y) x += held[zero + y];
+                    for (int y = 1 + thread % 8; y <= zero; y += 8) x += held[zero + y];
+            } else if (bucket < s.buckets) {
+                for (int y = max(from, 1) + thread % 8; y < to; y += 8) x += held[zero + y];
             }
-            g.table_part[(((static_cast<int64_t>(split) * a.batch + b) * column_tiles + column_tile) * a.heads + head) * s.buckets + bucket] = x;
+#pragma unroll
+            for (int i = 1; i < 8; i *= 2) x += __shfl_xor(x, i);
+            if (thread % 8 == 0 && bucket < s.buckets)
+                g.table_part[(((static_cast<int64_t>(split) * a.batch + b) * column_tiles + column_tile) * a.heads + head) * s.buckets + bucket] = x;
         }
     }
 }
@@ -329,15 +335,6 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
 
     if (__syncthreads_or(there)) {
         s16x8 kf[kSteps], vf[kSteps];
-        {
-            const int64_t k = row * a.k.outer + key * a.k.middle + kv_head * a.k.head;
-            const int64_t v = row * a.v.outer + key * a.v.middle + kv_head * a.v.head;
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                kf[i] = column(a.k, k, there, i, hi, a.d);
-                vf[i] = column(a.v, v, there, i, hi, a.d);
-            }
-        }
         const float scale_log2 = a.scale * kLog2e, by_scale = 1.f / a.scale;
         const int start = BIAS ? a.q_start_all + (a.q_start ? uniform(a.q_start[b]) : 0) : 0;
         Copier<DP, kQueries, 256> qs, ds;
@@ -370,6 +367,15 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
             }
         };
         load();
+        {
+            const int64_t k = row * a.k.outer + key * a.k.middle + kv_head * a.k.head;
+            const int64_t v = row * a.v.outer + key * a.v.middle + kv_head * a.v.head;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                kf[i] = column(a.k, k, there, i, hi, a.d);
+                vf[i] = column(a.v, v, there, i, hi, a.d);
+            }
+        }
         bool large = false;
         if constexpr (BIAS) {
             large = share > 1 && large_bias<E>(a.bias, head, share, a.scale, thread, 256);
@@ -537,12 +543,6 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
 
     if (__syncthreads_or(there)) {
         s16x8 own[kSteps];  // V or K
-        {
-            const AttendView& v = second ? a.v : a.k;
-            const int64_t at = row * v.outer + key * v.middle + kv_head * v.head;
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) own[i] = column(v, at, there, i, hi, a.d);
-        }
         const float scale_log2 = a.scale * kLog2e, by_scale = 1.f / a.scale;
         const int start = BIAS ? a.q_start_all + (a.q_start ? uniform(a.q_start[b]) : 0) : 0;
         const int query_tiles = (a.tokens + kQueries - 1) / kQueries, tiles = query_tiles * share;
@@ -592,6 +592,12 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         };
         int head = kv_head * share, first = 0;  // of the tile that is loaded next
         load(head, first);
+        {
+            const AttendView& v = second ? a.v : a.k;
+            const int64_t at = row * v.outer + key * v.middle + kv_head * v.head;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) own[i] = column(v, at, there, i, hi, a.d);
+        }
         bool large = false;
         if constexpr (BIAS) {
             large = share > 1 && large_bias<E>(a.bias, head, share, a.scale, thread, 512);

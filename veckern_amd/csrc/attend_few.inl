@@ -32,8 +32,6 @@ __global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(A
     const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
     char* mine = shared + wave * 2 * kTileBytes<DP, kFewKeys>;
     int2* found = reinterpret_cast<int2*>(shared + kFewTiles<DP>);
-    places.fill(a, b, found, thread, kThreads);
-
     const int c = column_tile * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
@@ -41,6 +39,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(A
     s16x8 qf[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
+    places.fill(a, b, found, thread, kThreads);
     const float* held = nullptr;
     int position = 0;
     if constexpr (BIAS) {

@@ -32,8 +32,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
     const int group = place % groups, b = place / groups;
     const int kv_head = group * a.pack / (a.heads / a.kv_heads);
 
-    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
-    places.fill(a, b, found, thread, 256);
     const int c = column_tile * kColumns + wave * 32 + lane % 32;
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
@@ -41,6 +39,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
     s16x8 qf[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
+    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
+    places.fill(a, b, found, thread, 256);
 
     f32x16 o[kParts];
 #pragma unroll
