@@ -94,14 +94,10 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     ks.init(thread, a.k.middle, a.d);
     vs.init(thread, a.v.middle, a.d);
     __syncthreads();
-    KeyWalk<kSlots> walk(places, found);
-    auto load = [&] {
-        ks.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
-        vs.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
-    };
+    KeyWalk<kSlots> walk(a, places, found, kv_head);
     bool more = walk.next();
     int now = 0;
-    if (more) load();  // before the biases: what they wait for is under way with it
+    if (more) walk.load(ks, vs);  // before the biases: what they wait for is under way with it
     int position = 0;
     float below = 0.f, above = 0.f;
     bool large = false;
@@ -164,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             for (int i = 0; i < kSlots; ++i) slots[i] = walk.slots[i];
             const bool full = walk.run || whole(slots);
             more = walk.next();
-            if (more) load();
+            if (more) walk.load(ks, vs);
             const int2 at_keys = reach(slots);
             k = tile[now][0];
             v = tile[now][1];

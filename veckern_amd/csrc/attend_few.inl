@@ -83,8 +83,8 @@ __global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(A
             at += kFewWaves * kSlots;
             step += (kFewWaves - 1) * kSlots;
             if (!any) continue;
-            ks.load(slots, false, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
-            vs.load(slots, false, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
+            ks.load(slots, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
+            vs.load(slots, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
             return true;
         }
         return false;

@@ -51,14 +51,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
     ks.init(thread, a.k.middle, a.d);
     vs.init(thread, a.v.middle, a.d);
     __syncthreads();
-    KeyWalk<kSlots> walk(places, found);
-    auto load = [&] {
-        ks.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.k, s, kv_head); });
-        vs.load(walk.slots, walk.run, [&](const Slot& s) { return slot_start(a.v, s, kv_head); });
-    };
+    KeyWalk<kSlots> walk(a, places, found, kv_head);
     bool more = walk.next();
     int now = 0;
-    if (more) load();  // before the biases: what they wait for is under way with it
+    if (more) walk.load(ks, vs);  // before the biases: what they wait for is under way with it
     const float* held = nullptr;
     int position = 0;
     bool large = false;
@@ -80,7 +76,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
             for (int i = 0; i < kSlots; ++i) slots[i] = walk.slots[i];
             const bool full = walk.run || whole(slots);
             more = walk.next();
-            if (more) load();
+            if (more) walk.load(ks, vs);
 
             f32x16 s[2] = {};
             float apart = 0.f;  // a bias that all keys of the tile share

@@ -102,10 +102,9 @@ struct Copier {
         step = static_cast<int>(stride * 2);
         to = thread / kChunks * kPitch<DP> + chunk * 16;
     }
-    // base(slot): where the slot's first row starts; run: the slots are full and follow each other in one row
+    // base(slot): where the slot's first row starts
     template <class F>
-    __device__ void load(const Slot (&slots)[ROWS / kSlot], bool run, F&& base) {
-        if (run) return load_rows(base(slots[0]), ROWS);
+    __device__ void load(const Slot (&slots)[ROWS / kSlot], F&& base) {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int at = wave_row + kRows * i, skipped = kRows * i % kSlot;
@@ -210,54 +209,78 @@ struct Places {
     }
 };
 
-// Walks the slots that hold a key, SLOTS at a time.
-template <int SLOTS>
-struct KeyWalk {
-    Slot slots[SLOTS];
-    bool run;  // the slots are full and follow each other in one row
-    const int2* found;
-    int per_row, end, r0, r, step, row, count;
-
-    __device__ KeyWalk(const Places& p, const int2* held) : found(held), per_row(p.per_row), end(p.end), r0(p.r0), r(p.r0) {
-        step = p.begin - p.r0 * per_row;
-        row = count = 0;
-        if (p.begin < end) take();
-        else r = end;
-    }
-    __device__ void take() {
-        row = uniform(found[r - r0].x);
-        count = uniform(found[r - r0].y);
-    }
-    // The next tile's slots, empty ones at the end; false where none is left.
-    __device__ bool next() {
-        const int first = step * kSlot;
-        run = count - first >= SLOTS * kSlot && r * per_row + step + SLOTS <= end;
-        if (run) {
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i) slots[i] = {row, first + kSlot * i, kSlot};
-            step += SLOTS;
-            return true;
-        }
-#pragma unroll
-        for (int i = 0; i < SLOTS; ++i) {
-            slots[i] = {0, 0, 0};
-            while (r * per_row + step < end) {
-                if (step * kSlot < count) {
-                    slots[i] = {row, step * kSlot, min(count - step * kSlot, kSlot)};
-                    ++step;
-                    break;
-                }
-                step = count = 0;
-                if (++r * per_row < end) take();
-            }
-        }
-        return slots[0].left > 0;
-    }
-};
 // Where a slot's first position starts, of a key head.
 __device__ __forceinline__ const char* slot_start(const AttendView& v, const Slot& s, int head) {
     return static_cast<const char*>(v.p) + (s.row * v.outer + s.first * v.middle + head * v.head) * 2;
 }
+// Walks the slots that hold a key, SLOTS at a time. While a row lasts its next tile is reached by adding to two addresses: what a
+// wave computes for itself between its tiles is on its critical path.
+template <int SLOTS>
+struct KeyWalk {
+    Slot slots[SLOTS];  // of the tile
+    bool run;           // they are full and follow each other in one row, from these addresses on
+    const char *k, *v;
+
+    const AttendArgs& a;
+    const int2* found;
+    int per_row, end, r0, head;
+    int r, row, first, left;  // the passage, its row, the next position and how many are left
+    const char *next_k, *next_v;
+
+    __device__ KeyWalk(const AttendArgs& args, const Places& p, const int2* held, int kv_head)
+        : a(args), found(held), per_row(p.per_row), end(p.end), r0(p.r0), head(kv_head), r(p.r0), row(0), first(0), left(0) {
+        next_k = next_v = nullptr;
+        if (p.begin < end) take((p.begin - p.r0 * per_row) * kSlot);
+        else r = end;
+    }
+    __device__ void take(int from) {
+        row = uniform(found[r - r0].x);
+        left = min(uniform(found[r - r0].y), (end - r * per_row) * kSlot) - from;
+        first = from;
+        next_k = slot_start(a.k, {row, first, 0}, head);
+        next_v = slot_start(a.v, {row, first, 0}, head);
+    }
+    __device__ void pass(int positions) {
+        first += positions;
+        left -= positions;
+        next_k += positions * a.k.middle * 2;
+        next_v += positions * a.v.middle * 2;
+    }
+    // Goes on to the next tile, empty slots at its end; false where none is left.
+    __device__ bool next() {
+        run = left >= SLOTS * kSlot;
+        if (run) {
+            k = next_k;
+            v = next_v;
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) slots[i] = {row, first + kSlot * i, kSlot};
+            pass(SLOTS * kSlot);
+            return true;
+        }
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            while (left <= 0 && r * per_row < end) {
+                if (++r * per_row < end) take(0);
+            }
+            slots[i] = {0, 0, 0};
+            if (left > 0) {
+                slots[i] = {row, first, min(left, kSlot)};
+                pass(kSlot);
+            }
+        }
+        return slots[0].left > 0;
+    }
+    template <class C>
+    __device__ void load(C& ks, C& vs) const {
+        if (run) {
+            ks.load_rows(k, SLOTS * kSlot);
+            vs.load_rows(v, SLOTS * kSlot);
+        } else {
+            ks.load(slots, [&](const Slot& s) { return slot_start(a.k, s, head); });
+            vs.load(slots, [&](const Slot& s) { return slot_start(a.v, s, head); });
+        }
+    }
+};
 // Whether all of a tile's places hold a key, and the first and last position of any.
 template <int SLOTS>
 __device__ __forceinline__ bool whole(const Slot (&s)[SLOTS]) {
