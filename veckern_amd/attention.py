@@ -129,13 +129,14 @@ def _arguments(q, keys, values, rows, lengths, bias, q_start, scale) -> _Attenti
     return a
 
 
-class _Plan(NamedTuple):
+class _Plan:
     """What calls with the same sizes, strides, types and devices share: the arguments but for the addresses."""
 
-    image: bytes
-    forward_bytes: int
-    backward_bytes: int
-    lse_shape: tuple
+    __slots__ = ("image", "forward_bytes", "backward_bytes", "lse_shape", "grads")
+
+    def __init__(self, image, forward_bytes, backward_bytes, lse_shape):
+        self.image, self.forward_bytes, self.backward_bytes, self.lse_shape = image, forward_bytes, backward_bytes, lse_shape
+        self.grads = {}  # by the kinds of what the backward pass is given besides: the gradients' strides
 
 
 _plans: dict = {}
@@ -165,8 +166,14 @@ def _plan(q, keys, values, rows, lengths, bias, q_start, scale) -> _Plan:
 
 _ADDRESS = struct.Struct("P")
 _AT = {name: getattr(_Attention, name).offset for name in ("q", "k", "v", "out", "rows", "lengths", "lse", "table", "q_starts")}
+_GRAD_AT = {name: getattr(_AttentionGrad, name).offset for name in ("d_q", "d_k", "d_v", "d_table")}
 _OUT_STRIDE = _AT["out"] + _Tensor.stride.offset
 _STRIDES = struct.Struct("3q")
+
+
+def _contiguous(shape) -> tuple:
+    _, b, c, d = shape
+    return (b * c * d, c * d, d)
 
 
 def _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start) -> _Attention:
@@ -267,26 +274,32 @@ def attend_backward(d_out: torch.Tensor, q: torch.Tensor, keys: torch.Tensor, va
     """The gradients of a loss whose gradient by ``out`` is ``d_out``; ``out`` and ``lse`` as ``attend`` returned them for
     the same arguments. With ``rows`` the bank is a constant and has none."""
     plan = _plan(q, keys, values, rows, lengths, bias, q_start, scale)
-    if lse.shape != plan.lse_shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
-        _refuse(f"lse must be contiguous {list(plan.lse_shape)} float32 on {q.device}")
-    _view(out, "out", q.shape, q)
+    kind = (_kind(d_out), _kind(out), _kind(lse))
+    grads = plan.grads.get(kind)
+    if grads is None:
+        if lse.shape != plan.lse_shape or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+            _refuse(f"lse must be contiguous {list(plan.lse_shape)} float32 on {q.device}")
+        _view(out, "out", q.shape, q)
+        g = _AttentionGrad()
+        g.d_out = _view(d_out, "d_out", q.shape, q)
+        g.d_q.stride = _contiguous(q.shape)
+        g.d_k.stride = g.d_v.stride = _contiguous(keys.shape)
+        if len(plan.grads) >= _MOST_PLANS:
+            plan.grads.clear()
+        grads = plan.grads[kind] = bytes(g)
     a = _filled(plan, q, keys, values, out, lse, rows, lengths, bias, q_start)
-    g = _AttentionGrad()
-    g.d_out = _view(d_out, "d_out", q.shape, q)
-
-    def like(t):
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-    def whole(t):
-        return _Tensor(t.data_ptr(), t.stride()[:3])
-
-    d_q, d_k, d_v, d_table = like(q), None, None, None
-    g.d_q = whole(d_q)
+    g, put = bytearray(grads), _ADDRESS.pack_into
+    d_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    d_k = d_v = d_table = None
+    put(g, 0, d_out.data_ptr())
+    put(g, _GRAD_AT["d_q"], d_q.data_ptr())
     if rows is None:
-        d_k, d_v = like(keys), like(values)
-        g.d_k, g.d_v = whole(d_k), whole(d_v)
+        d_k = torch.empty(keys.shape, dtype=q.dtype, device=q.device)
+        d_v = torch.empty(keys.shape, dtype=q.dtype, device=q.device)
+        put(g, _GRAD_AT["d_k"], d_k.data_ptr())
+        put(g, _GRAD_AT["d_v"], d_v.data_ptr())
     if bias is not None:
-        d_table = like(bias.table)
-        g.d_table = d_table.data_ptr()
-    _launch(library().vk_attend_backward, (a, g), plan.backward_bytes, q.device)
+        d_table = torch.empty(bias.table.shape, dtype=q.dtype, device=q.device)
+        put(g, _GRAD_AT["d_table"], d_table.data_ptr())
+    _launch(library().vk_attend_backward, (a, _AttentionGrad.from_buffer(g)), plan.backward_bytes, q.device)
     return Gradients(d_q, d_k, d_v, d_table)
