@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
         for (int sub = 0; sub < kSubs; ++sub) {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
+                if (i) s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
                 dp[sub] = E::mfma(straight<DP>(v, 32 * sub, i, lane), df[i], dp[sub]);
             }
         }
@@ -164,27 +164,30 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
             const int2 at_keys = reach(slots);
             k = tile[now][0];
             v = tile[now][1];
-            f32x16 s[kSubs] = {}, dp[kSubs] = {};
+            f32x16 s[kSubs], dp[kSubs] = {};
             bool near = kLarge;  // the tile's keys do not share one bias
             float apart = 0.f;   // the bias they share
             int t0 = 0;
             if constexpr (BIAS) {
                 t0 = __builtin_amdgcn_readfirstlane(position);
-                if (!kLarge) {
-                    near = !far_apart(a.bias, at_keys.x - (t0 + 31), at_keys.y - t0);
-                    if (near) {
+                if (!kLarge) near = !far_apart(a.bias, at_keys.x - (t0 + 31), at_keys.y - t0);
+            }
+            // the first product of each sum stands in the branch: beginning with zero costs no instruction there
+            if (BIAS && !kLarge && near) {
 #pragma unroll
-                        for (int sub = 0; sub < kSubs; ++sub)
-                            each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
-                                         [&](int r, float x) { s[sub][r] = x; });
-                    } else {
-                        apart = held[bias_index(a.bias.far, at_keys.x - position)] * a.scale;
-                    }
+                for (int sub = 0; sub < kSubs; ++sub) {
+                    each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
+                                 [&](int r, float x) { s[sub][r] = x; });
+                    s[sub] = E::mfma(straight<DP>(k, 32 * sub, 0, lane), qf[0], s[sub]);
                 }
+            } else {
+                if (BIAS && !kLarge) apart = held[bias_index(a.bias.far, at_keys.x - position)] * a.scale;
+#pragma unroll
+                for (int sub = 0; sub < kSubs; ++sub) s[sub] = E::mfma(straight<DP>(k, 32 * sub, 0, lane), qf[0], f32x16{});
             }
             between_runs();
             products(s, dp);
-            feed<2 * kSubs * kSteps, 1, 4>();
+            feed<2 * kSubs * kSteps - kSubs, 1, 4>();
             between_runs();
             if constexpr (kLarge) {
 #pragma unroll

@@ -78,28 +78,37 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
             more = walk.next();
             if (more) walk.load(ks, vs);
 
-            f32x16 s[2] = {};
+            f32x16 s[2];
+            const char *k = tile[now][0], *v = tile[now][1];
             float apart = 0.f;  // a bias that all keys of the tile share
+            bool near = false;  // the tile's keys do not share one bias
+            int2 at{};
             if constexpr (BIAS && !kLarge) {
                 // the wave's tokens lie between its first and last column's
                 const int t0 = __builtin_amdgcn_readfirstlane(position), t1 = __builtin_amdgcn_readlane(position, 31);
-                const int2 at = reach(slots);
-                if (far_apart(a.bias, at.x - t1, at.y - t0)) {
-                    apart = held[bias_index(a.bias.far, at.x - position)] * a.scale;
-                } else {
-#pragma unroll
-                    for (int sub = 0; sub < 2; ++sub)
-                        each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
-                                     [&](int r, float x) { s[sub][r] = x; });
-                }
+                at = reach(slots);
+                near = !far_apart(a.bias, at.x - t1, at.y - t0);
             }
             __builtin_amdgcn_s_setprio(1);
+            // the first product of each sum stands in the branch: beginning with zero costs no instruction there
+            if (BIAS && near) {
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) {
+                    each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
+                                 [&](int r, float x) { s[sub][r] = x; });
+                    s[sub] = E::mfma(straight<DP>(k, 32 * sub, 0, lane), qf[0], s[sub]);
+                }
+            } else {
+                if (BIAS && !kLarge) apart = held[bias_index(a.bias.far, at.x - position)] * a.scale;
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) s[sub] = E::mfma(straight<DP>(k, 32 * sub, 0, lane), qf[0], f32x16{});
+            }
             between_runs();
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(tile[now][0], 32 * sub, i, lane), qf[i], s[sub]);
-            feed<2 * kSteps, 1, 4>();
+                for (int i = 1; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
+            feed<2 * kSteps - 2, 1, 4>();
             between_runs();
             __builtin_amdgcn_s_setprio(0);
             if constexpr (kLarge) {
@@ -143,7 +152,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
             for (int half = 0; half < 4; ++half) {
                 const s16x8 p = rounded<E>(s[half / 2], half % 2);
 #pragma unroll
-                for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(tile[now][1], 16 * half, i, lane), p, o[i]);
+                for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(v, 16 * half, i, lane), p, o[i]);
             }
             feed<4 * kParts, 2, 4>();
             between_runs();
