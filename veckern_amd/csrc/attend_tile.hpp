@@ -111,8 +111,12 @@ struct Copier {
             Slot s = slots[kRows * i / kSlot];
             if constexpr (kRows > kSlot) {  // the waves of a step copy different slots
 #pragma unroll
-                for (int j = kRows * i / kSlot + 1; j < kRows * (i + 1) / kSlot; ++j)
-                    if (at / kSlot == j) s = slots[j];
+                for (int j = kRows * i / kSlot + 1; j < kRows * (i + 1) / kSlot; ++j) {
+                    const bool here = at / kSlot == j;
+                    s.row = here ? slots[j].row : s.row;
+                    s.first = here ? slots[j].first : s.first;
+                    s.left = here ? slots[j].left : s.left;
+                }
             }
             auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base(s)), 0, 0x7fffffff, 0x00020000);
             held[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, row + skipped < s.left ? offset + step * skipped : kOut, 0, 0);
