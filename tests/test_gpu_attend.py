@@ -109,6 +109,36 @@ def test_position_bias(shape, kind, dtype):
     both(q, k, v, rows, lengths, table, buckets, max_distance, two_sided, start, d_out=d_out)
 
 
+@pytest.mark.parametrize("two_sided", [True, False])
+@pytest.mark.parametrize("d", [32, 64, 80, 128])
+def test_wide_position_bias_over_many_blocks(d, two_sided):
+    """More blocks than compute units, and buckets so wide that the table's gradient is summed without a tile in LDS."""
+    batch, tokens, heads = 34, 9, 8
+    q, k, v, _, lengths, d_out = make(d, BF16, batch, tokens, 3, 70, heads, 4, d, 0, True)
+    table = torch.randn(64, heads, generator=torch.Generator().manual_seed(d)).to(BF16).cuda()
+    both(q, k, v, lengths=lengths, table=table, buckets=64, max_distance=512, two_sided=two_sided, q_start=35, d_out=d_out)
+
+
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("shape", [(1, 900, 2, 40, 8, 2, 64, 0, True), (1, 1100, 1, 50, 4, 4, 24, 0, False),
+                                   (1, 700, 3, 33, 8, 2, 128, 0, True), (2, 515, 1, 19, 6, 2, 96, 0, False)], ids=str)
+def test_many_tokens_over_few_states(shape, biased):
+    """The states' gradient is summed over query tiles by several blocks."""
+    q, k, v, _, lengths, d_out = make(31, BF16, *shape)
+    bias = {}
+    if biased:
+        table = torch.randn(32, shape[4], generator=torch.Generator().manual_seed(32)).to(BF16).cuda()
+        bias = dict(table=table, buckets=32, max_distance=128, two_sided=True)
+    both(q, k, v, lengths=lengths, d_out=d_out, **bias)
+
+
+@pytest.mark.parametrize("shape", [(2, 150, 5, 23, 4, 2, 32, 12, True), (3, 40, 9, 7, 2, 2, 16, 0, True),
+                                   (1, 300, 1, 190, 2, 1, 24, 0, False)], ids=str)
+def test_small_heads(shape):
+    q, k, v, rows, lengths, d_out = make(41, F16, *shape)
+    both(q, k, v, rows=rows, lengths=lengths, d_out=d_out)
+
+
 @pytest.mark.parametrize("start", [-700, -1, 3, 90, 5000])
 def test_position_of_the_first_token(start):
     q, k, v, _, _, d_out = make(13, BF16, 1, 66, 2, 100, 2, 2, 64)

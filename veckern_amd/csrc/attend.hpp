@@ -17,7 +17,10 @@ constexpr int kKeyTile = 64;         // keys that a block of the tile kernels ho
 constexpr int kFewWaves = 8, kFewKeys = 32;  // waves of a block of the few-columns kernel, keys of its tiles
 constexpr int kHeldPassages = 256;   // passages that a block holds the rows of
 constexpr int grad_keys(int d) { return d <= 64 ? 64 : 32; }  // keys of a tile of the query gradient
+constexpr int grad_queries(int d) { return d <= 64 ? 64 : 32; }  // queries of a tile of the keys' and values' gradient
 constexpr int kColumns = 128;        // query columns of a block of the tile kernels
+constexpr int kUnits = 256;          // compute units of the card
+constexpr int kLds = 160 * 1024;     // LDS of a compute unit
 
 // A tensor [outer][middle][head][d]: element strides, d contiguous.
 struct AttendView {
@@ -62,6 +65,9 @@ struct AttendGradArgs {
     float* delta = nullptr;       // workspace [batch][heads][tokens]
     float* table_part = nullptr;  // workspace [splits * batch * column tiles][heads][buckets]
     void* d_table = nullptr;      // [buckets][heads], contiguous
+    // Runs of a key head's query tiles (head by head) that different blocks take for d_k and d_v.
+    int kv_splits = 1, kv_tiles_per_split = 0;
+    float* kv_part = nullptr;     // kv_splits > 1: workspace [d_k, d_v][kv_splits][bank][length][kv_heads][d]
 };
 
 enum AttendType { kAttendF16 = 0, kAttendBf16 = 1 };
@@ -72,7 +78,7 @@ hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stre
 // Writes d_q, or its parts, delta and the table's partial sums.
 hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream);
 hipError_t launch_attend_grad_kv(const AttendGradArgs& g, int type, hipStream_t stream);
-// Joins what grad_q's splits wrote, and the table's partial sums.
+// Joins what the splits wrote, and the table's partial sums.
 hipError_t launch_attend_grad_join(const AttendGradArgs& g, int type, int parts, hipStream_t stream);
 
 }  // namespace vk

@@ -21,27 +21,54 @@ __device__ __forceinline__ void store_four(void* p, int at, const f32x16& x, int
 }
 
 // Adds dS of a 32 x 32 tile (lane: one query position, x: the distance of the tile's first key from the first query) to a
-// wave's sums by distance, in a fixed order. The tile goes through LDS by diagonals: element (key, query) to row 31 + key -
-// query and place `query` of `skew`, whose other places stay zero; then a lane sums one diagonal and adds it to that distance's
-// place, or, beyond the far ends, to a register. With 36 floats a row neither the writes nor the 16-byte reads share a bank. (Adding each element to its distance's place by an LDS atomic took 130
-// clocks an instruction.)
+// wave's sums by distance, in a fixed order, in one of two ways; past the ends of the buckets a sum goes to a register. (An LDS
+// atomic for each element took 130 clocks an instruction.)
+//   skewed: the tile goes through LDS by diagonals, element (key, query) to row 31 + key - query and place `query` of `skew`,
+//     whose other places stay zero; then a lane sums one diagonal. With 36 floats a row neither the writes nor the 16-byte reads
+//     share a bank.
+//   turned: of each result, rows n and n + 1 in the two halves of the wave, the queries are turned by n lanes within a half:
+//     then lane j has the distances -j and 32 - j of every row (one more in the upper half), and adds what it is given to one of
+//     two sums.
+// The first takes fewer instructions (32 requests of 512 tokens, 64 elements, far 91: 99 us against 110), but 36 KB a block: where
+// two blocks of a compute unit then have no room, the second is faster (26 requests of 714 tokens and 162 keys, far 469: 104 us
+// against 76).
 constexpr int kSkew = 36, kSkewFloats = 63 * kSkew;
-__device__ __forceinline__ void put_diagonals(const f32x16& ds, float* skew, int lane) {
-    float* to = skew + (31 - lane % 32 + lane / 32) * kSkew + lane % 32;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) to[tile_row(r, 0) * kSkew] = ds[r];
-    between_lanes();
+template <int R>
+__device__ __forceinline__ void turn(const f32x16& ds, int lane, float& near, float& further) {
+    constexpr int n = tile_row(R, 0), kTurn = 0xc000 | n << 5;  // lane j of 32 reads lane (j + n) % 32
+    const float x = n ? __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(ds[R]), kTurn)) : ds[R];
+    const bool turned = lane % 32 >= 32 - n;
+    near += turned ? 0.f : x;
+    if (n) further += turned ? x : 0.f;
+    if constexpr (R < 15) turn<R + 1>(ds, lane, near, further);
 }
-__device__ __forceinline__ void sum_diagonals(const float* skew, float* sums, int far, int x, int lane, float& below, float& above) {
-    const f32x4* from = reinterpret_cast<const f32x4*>(skew + min(lane, 62) * kSkew);
-    f32x4 y = from[0];
+template <bool SKEWED>
+__device__ __forceinline__ void add_diagonals(const f32x16& ds, float* skew, float* sums, int far, int x, int lane, float& below, float& above) {
+    float sum;
+    int distance;
+    if constexpr (SKEWED) {
+        float* to = skew + (31 - lane % 32 + lane / 32) * kSkew + lane % 32;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) y += from[i];
-    const float all = lane < 63 ? (y[0] + y[1]) + (y[2] + y[3]) : 0.f;
-    const int place = x + lane - 31 + far + kPad;
-    if (place < 0) below += all;
-    else if (place > 2 * far + 2 * kPad) above += all;
-    else if (lane < 63) sums[place] += all;
+        for (int r = 0; r < 16; ++r) to[tile_row(r, 0) * kSkew] = ds[r];
+        between_lanes();
+        const f32x4* from = reinterpret_cast<const f32x4*>(skew + min(lane, 62) * kSkew);
+        f32x4 y = from[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) y += from[i];
+        sum = lane < 63 ? (y[0] + y[1]) + (y[2] + y[3]) : 0.f;
+        distance = x + lane - 31;
+    } else {
+        float near = 0.f, further = 0.f;  // distance -j and 32 - j
+        turn<0>(ds, lane, near, further);
+        // both sums of the lower half, and beside them those of the upper half, which belong to the lane before
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(near), __float_as_uint(further), false, false);
+        sum = __uint_as_float(y[0]) + __int_as_float(__builtin_amdgcn_ds_bpermute((lane + 1) % 64 * 4, y[1]));
+        distance = x - lane % 32 + (lane & 32);
+    }
+    const int place = distance + far + kPad;
+    if (place < 0) below += sum;
+    else if (place > 2 * far + 2 * kPad) above += sum;
+    else if (!SKEWED || lane < 63) sums[place] += sum;
     between_lanes();
 }
 
@@ -51,9 +78,13 @@ __device__ __forceinline__ int bucket_begin(const AttendBias& s, int j) {
     return j <= exact ? j : j - exact - 1 < s.edges ? s.edge[j - exact - 1] : s.far + kPad + 1;
 }
 
-template <class E, int DP, bool BIAS>
+// How the table's gradient is summed, if there is one.
+enum TableSums { kNoTable, kSkewedSums, kTurnedSums };
+
+template <class E, int DP, TableSums SUMS>
 __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     // with 128 elements a head two waves a SIMD have no registers for more
+    constexpr bool BIAS = SUMS != kNoTable, kSkewed = SUMS == kSkewedSums;
     constexpr int kSteps = DP / 16, kParts = DP / 32, kKeys = grad_keys(DP), kSubs = kKeys / 32, kSlots = kKeys / kSlot;
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeys>];
@@ -105,10 +136,11 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     if constexpr (BIAS) {
         const int distances = bias_places(a.bias.far);
         skew = shared + wave * kSkewFloats;
-        held = shared + 4 * kSkewFloats;
+        held = shared + (kSkewed ? 4 * kSkewFloats : 0);
         sums = held + (1 + wave) * distances;
         large = fill_biases<E>(a.bias, head, 1, a.scale, held, thread, 256);
-        for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
+        if constexpr (kSkewed)
+            for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
         for (int i = thread; i < 4 * distances; i += 256) held[distances + i] = 0.f;
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
@@ -217,16 +249,14 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
                             f32x16 one = s[sub];
 #pragma unroll
                             for (int r = 0; r < 8; ++r) one[r] = 0.f;
-                            put_diagonals(one, skew, lane);
-                            sum_diagonals(skew, sums, a.bias.far, y.first - kSlot - t0, lane, below, above);
+                            add_diagonals<kSkewed>(one, skew, sums, a.bias.far, y.first - kSlot - t0, lane, below, above);
                             one = s[sub];
 #pragma unroll
                             for (int r = 8; r < 16; ++r) one[r] = 0.f;
-                            put_diagonals(one, skew, lane);
+                            add_diagonals<kSkewed>(one, skew, sums, a.bias.far, x.first - t0, lane, below, above);
                         } else {
-                            put_diagonals(s[sub], skew, lane);
+                            add_diagonals<kSkewed>(s[sub], skew, sums, a.bias.far, x.first - t0, lane, below, above);
                         }
-                        sum_diagonals(skew, sums, a.bias.far, x.first - t0, lane, below, above);
                     }
                 } else {
                     float all = 0.f;
@@ -303,10 +333,38 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     }
 }
 
+// Writes a key's d_k or d_v, or a split's part of it. Keys past the row's length have no gradient: zeros.
+template <class E, int DP>
+__device__ __forceinline__ void store_key(const AttendGradArgs& g, bool value, int split, int row, int key, int kv_head, int hi, bool there,
+                                          const f32x16 (&sum)[DP / 32]) {
+    const AttendArgs& a = g.a;
+    const AttendView& v = value ? g.d_v : g.d_k;
+    const f32x16 zero{};
+    auto each = [&](auto&& store) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int quad = 0; quad < 4; ++quad) {
+                const int e = 32 * i + mfma_row(4 * quad, hi);
+                if (e < a.d) store(e, there ? sum[i] : zero, quad);
+            }
+    };
+    if (g.kv_splits > 1) {
+        float* part = g.kv_part + ((((value ? g.kv_splits : 0) + split) * a.bank + row) * a.length + key) * a.kv_heads * a.d + kv_head * a.d;
+        each([&](int e, const f32x16& x, int quad) {
+            *reinterpret_cast<f32x4*>(part + e) = f32x4{x[4 * quad], x[4 * quad + 1], x[4 * quad + 2], x[4 * quad + 3]};
+        });
+    } else {
+        char* out = static_cast<char*>(v.p) + (row * v.outer + key * v.middle + kv_head * v.head) * 2;
+        const float factor = value ? 1.f : g.scale;
+        each([&](int e, const f32x16& x, int quad) { store_four<typename E::T>(out, e, x, quad, factor); });
+    }
+}
+
 // One block: 128 keys of a request and key head (8 slots), each wave 32 of them; walks the request's query tiles, head by head.
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
-    constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = 64;
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = grad_queries(DP);
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kQueries>];
     // of each query, in the order of the products' rows: -lse / scale and -delta, with which the products' sums begin; for
@@ -320,6 +378,11 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
     int place = xcd_place(blockIdx.x, gridDim.x);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
+    int split = 0;
+    if (g.kv_splits > 1) {
+        split = place % g.kv_splits;
+        place /= g.kv_splits;
+    }
     const int kv_head = place % a.kv_heads, b = place / a.kv_heads;
     // the lane's key, by slots: of the passages of a request, 16 positions each
     const int slot = key_tile * (kColumns / kSlot) + wave * 2 + lane % 32 / kSlot, passage = slot / per_row;
@@ -341,7 +404,13 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         ds.init(thread, g.d_out.middle, a.d);
         float2 lse;
         float delta = 0.f;
+        const int query_tiles = (a.tokens + kQueries - 1) / kQueries, begin = split * g.kv_tiles_per_split;
+        int left = min(g.kv_tiles_per_split, query_tiles * share - begin);  // tiles
         int head = kv_head * share, first = 0;
+        if (split) {
+            head += begin / query_tiles;
+            first = begin % query_tiles * kQueries;
+        }
         auto load = [&] {
             const int valid = a.tokens - first;
             qs.load_rows(slot_start(a.q, {b, first, 0}, head), valid);
@@ -377,14 +446,14 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         }
         bool large = false;
         if constexpr (BIAS) {
-            large = share > 1 && large_bias<E>(a.bias, head, share, a.scale, thread, 256);
+            large = share > 1 && large_bias<E>(a.bias, kv_head * share, share, a.scale, thread, 256);
             if (large) fill_bias<E>(a.bias, head, 1.f, bias_held, thread, 256);
             else large = fill_biases<E>(a.bias, head, 1, a.scale, bias_held, thread, 256);
         }
         store(0);
         __syncthreads();
         int now = 0;
-        bool more = true;
+        bool more = left > 0;
         const char *q, *d;
         auto of = [&](int which, int sub, int quad) {
             return *reinterpret_cast<const f32x4*>(&stat[now][which][32 * sub + mfma_row(4 * quad, hi)]);
@@ -421,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                     ++head;
                     turned = true;
                 }
-                more = head < (kv_head + 1) * share;
+                more = --left > 0;
                 if (more) load();
                 q = tile[now][0];
                 d = tile[now][1];
@@ -489,19 +558,9 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         else run(std::false_type());
     }
 
-    if (inside && key < a.length) {  // keys past the row's length have no gradient: zeros
-        char* k = static_cast<char*>(g.d_k.p) + (row * g.d_k.outer + key * g.d_k.middle + kv_head * g.d_k.head) * 2;
-        char* v = static_cast<char*>(g.d_v.p) + (row * g.d_v.outer + key * g.d_v.middle + kv_head * g.d_v.head) * 2;
-#pragma unroll
-        for (int i = 0; i < kParts; ++i)
-#pragma unroll
-            for (int quad = 0; quad < 4; ++quad) {
-                const int e = 32 * i + mfma_row(4 * quad, hi);
-                if (e >= a.d) continue;
-                const f32x16 zero{};
-                store_four<typename E::T>(k, e, there ? dk[i] : zero, quad, g.scale);
-                store_four<typename E::T>(v, e, there ? dv[i] : zero, quad, 1.f);
-            }
+    if (inside && key < a.length) {
+        store_key<E, DP>(g, false, split, row, key, kv_head, hi, there, dk);
+        store_key<E, DP>(g, true, split, row, key, kv_head, hi, there, dv);
     }
 }
 
@@ -512,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
 // Both take as many products; three tiles lie in LDS, one for each of them and one to be filled.
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) {
-    constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = 32;
+    constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = grad_queries(DP);
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[3][2][kTileBytes<DP, kQueries>];
     __shared__ f32x4 handed[2][4][4][64];  // P of a tile: by waves, quads of rows, lanes
@@ -528,6 +587,11 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
     int place = xcd_place(blockIdx.x, gridDim.x);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
+    int split = 0;
+    if (g.kv_splits > 1) {
+        split = place % g.kv_splits;
+        place /= g.kv_splits;
+    }
     const int kv_head = place % a.kv_heads, b = place / a.kv_heads;
     // the lane's key, by slots: of the passages of a request, 16 positions each
     const int slot = key_tile * (kColumns / kSlot) + wave * 2 + lane % 32 / kSlot, passage = slot / per_row;
@@ -544,7 +608,8 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         s16x8 own[kSteps];  // V or K
         const float scale_log2 = a.scale * kLog2e, by_scale = 1.f / a.scale;
         const int start = BIAS ? a.q_start_all + (a.q_start ? uniform(a.q_start[b]) : 0) : 0;
-        const int query_tiles = (a.tokens + kQueries - 1) / kQueries, tiles = query_tiles * share;
+        const int query_tiles = (a.tokens + kQueries - 1) / kQueries, first_tile = split * g.kv_tiles_per_split;
+        const int tiles = min(g.kv_tiles_per_split, query_tiles * share - first_tile);
         const AttendView& rows = second ? g.d_out : a.q;  // each half of the block copies one of the two
         Copier<DP, kQueries, 256> copier;
         copier.init(thread % 256, rows.middle, a.d);
@@ -590,6 +655,10 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
             feed<2 * kParts, 2, 3>();
         };
         int head = kv_head * share, first = 0;  // of the tile that is loaded next
+        if (split) {
+            head += first_tile / query_tiles;
+            first = first_tile % query_tiles * kQueries;
+        }
         load(head, first);
         {
             const AttendView& v = second ? a.v : a.k;
@@ -599,7 +668,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         }
         bool large = false;
         if constexpr (BIAS) {
-            large = share > 1 && large_bias<E>(a.bias, head, share, a.scale, thread, 512);
+            large = share > 1 && large_bias<E>(a.bias, kv_head * share, share, a.scale, thread, 512);
             if (large) fill_bias<E>(a.bias, head, 1.f, bias_held, thread, 512);
             else large = fill_biases<E>(a.bias, head, 1, a.scale, bias_held, thread, 512);
         }
@@ -684,20 +753,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         else both(std::false_type());
     }
 
-    if (inside && key < a.length) {  // keys past the row's length have no gradient: zeros
-        const AttendView& v = second ? g.d_k : g.d_v;
-        char* out = static_cast<char*>(v.p) + (row * v.outer + key * v.middle + kv_head * v.head) * 2;
-        const float factor = second ? g.scale : 1.f;
-#pragma unroll
-        for (int i = 0; i < kParts; ++i)
-#pragma unroll
-            for (int quad = 0; quad < 4; ++quad) {
-                const int e = 32 * i + mfma_row(4 * quad, hi);
-                if (e >= a.d) continue;
-                const f32x16 zero{};
-                store_four<typename E::T>(out, e, there ? sum[i] : zero, quad, factor);
-            }
-    }
+    if (inside && key < a.length) store_key<E, DP>(g, !second, split, row, key, kv_head, hi, there, sum);
 }
 
 template <class E, int DP>
@@ -705,8 +761,14 @@ hipError_t launch_grad_q(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns * (a.heads / a.pack) * a.batch * a.splits;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    const size_t lds = a.bias.table ? (4 * kSkewFloats + 5 * (2 * a.bias.far + 2 * kPad + 1)) * sizeof(float) : 0;
-    auto kernel = a.bias.table ? grad_q_kernel<E, DP, true> : grad_q_kernel<E, DP, false>;
+    size_t lds = a.bias.table ? 5 * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
+    auto kernel = a.bias.table ? grad_q_kernel<E, DP, kTurnedSums> : grad_q_kernel<E, DP, kNoTable>;
+    constexpr size_t kSkewed = 4 * kSkewFloats * sizeof(float),
+                     kOwn = 4 * kTileBytes<DP, grad_keys(DP)> + kHeldPassages * sizeof(int2) + 256;  // 256: of __syncthreads_or
+    if (a.bias.table && (blocks <= kUnits || 2 * (kOwn + kSkewed + lds) <= kLds)) {
+        kernel = grad_q_kernel<E, DP, kSkewedSums>;
+        lds += kSkewed;
+    }
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
     return hipGetLastError();
 }
@@ -715,7 +777,7 @@ template <class E, int DP>
 hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t slots = static_cast<int64_t>((a.length + kSlot - 1) / kSlot) * a.passages;
-    const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch;
+    const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch * g.kv_splits;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     if constexpr (DP <= 64) {  // two waves for 32 keys: 170 us where one takes 142 (4 x 2048 tokens, 12 heads of 64)

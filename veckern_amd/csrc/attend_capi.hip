@@ -166,8 +166,6 @@ AttendArgs args_of(const vk_attention* x, bool tensors) {
     return a;
 }
 
-constexpr int64_t kUnits = 256;  // compute units of the card
-
 // Whether a call has so few columns for each key head that its time is the reading of the states.
 bool few_columns(const AttendArgs& a) { return static_cast<int64_t>(a.tokens) * a.pack <= 32; }
 
@@ -178,33 +176,36 @@ struct Pace {
     double start, tile, shared;
 };
 
-// Splits the keys into runs of whole tiles, for different blocks, where that makes a call shorter: the runs' parts are joined by
-// another launch (5 us) that reads what the runs wrote in 32 bits (3.5 TB/s). At the pace of the tile kernel one split of 256
+// Into how many runs of whole tiles, for different blocks, an axis of `tiles` tiles is split where that makes a call shorter: the
+// runs' parts are joined by another launch (5 us) that reads what the runs wrote in 32 bits (part_bytes a run, both ways, at
+// 3.5 TB/s). `blocks`: of one run; at_a_time: tiles that a block takes at once. At the pace of the tile kernel one split of 256
 // blocks over 80 tiles of 64 elements a head took 107 us, two 75 + 6 and three, which fill the card, 63 + 7; of 18 blocks over 15
 // tiles of 128, one 26 us, five 12 + 4 and fifteen 12 + 7.
+int best_splits(int tiles, int least, int64_t blocks, const Pace& pace, int at_a_time, double part_bytes) {
+    double best = 0;
+    int splits = 1;
+    for (int s = least; s <= std::max(least, std::min(tiles, 64)); ++s) {
+        const int each = (tiles + s - 1) / s;
+        if (s > least && (tiles + each - 1) / each != s) continue;
+        const int64_t all = blocks * s, beside = std::max<int64_t>(1, std::min<int64_t>(pace.resident, (all + vk::kUnits - 1) / vk::kUnits));
+        const double rounds = static_cast<double>((all + vk::kUnits * beside - 1) / (vk::kUnits * beside));
+        const double time = rounds * (pace.start + (each + at_a_time - 1) / at_a_time * pace.tile * (1 + pace.shared * (beside - 1))) +
+                            (s > 1 ? 5 + s * part_bytes / 3.5e6 : 0);
+        if (s == least || time < best) {
+            best = time;
+            splits = each ? (tiles + each - 1) / each : 1;
+        }
+    }
+    return splits;
+}
 void split_keys(AttendArgs& a, int keys, int64_t blocks, const Pace& pace, int at_a_time) {
-    const double part_bytes = 8.0 * a.batch * a.heads * a.tokens * a.d;
     const int per_row = (a.length + vk::kSlot - 1) / vk::kSlot, per_tile = keys / vk::kSlot;
     const int tiles = static_cast<int>((static_cast<int64_t>(per_row) * a.passages + per_tile - 1) / per_tile);
     // a block holds the rows of kHeldPassages passages, and a run touches one more than it fills
     const int64_t most_tiles = std::max<int64_t>(1, static_cast<int64_t>(vk::kHeldPassages - 1) * per_row / per_tile);
     const int least = static_cast<int>(std::max<int64_t>(1, (tiles + most_tiles - 1) / most_tiles));
-    double best = 0;
-    a.splits = 1;
-    a.tiles_per_split = tiles;
-    for (int s = least; s <= std::max(least, std::min(tiles, 64)); ++s) {
-        const int each = (tiles + s - 1) / s;
-        if (s > least && (tiles + each - 1) / each != s) continue;
-        const int64_t all = blocks * s, beside = std::max<int64_t>(1, std::min<int64_t>(pace.resident, (all + kUnits - 1) / kUnits));
-        const double rounds = static_cast<double>((all + kUnits * beside - 1) / (kUnits * beside));
-        const double time = rounds * (pace.start + (each + at_a_time - 1) / at_a_time * pace.tile * (1 + pace.shared * (beside - 1))) +
-                            (s > 1 ? 5 + s * part_bytes / 3.5e6 : 0);
-        if (s == least || time < best) {
-            best = time;
-            a.splits = each ? (tiles + each - 1) / each : 1;
-            a.tiles_per_split = each;
-        }
-    }
+    a.splits = best_splits(tiles, least, blocks, pace, at_a_time, 8.0 * a.batch * a.heads * a.tokens * a.d);
+    a.tiles_per_split = (tiles + a.splits - 1) / a.splits;
 }
 
 void plan_forward(AttendArgs& a) {
@@ -220,24 +221,35 @@ void plan_forward(AttendArgs& a) {
                    small ? Pace{3, 6, 1.27, 0.34} : Pace{2, 6, 1.33, 0.66}, 1);
     }
 }
-void plan_backward(AttendArgs& a) {
+void plan_backward(AttendGradArgs& g) {
+    AttendArgs& a = g.a;
     a.pack = a.bias.table ? 1 : a.heads / a.kv_heads;
     const int64_t columns = static_cast<int64_t>(a.tokens) * a.pack, rest = static_cast<int64_t>(a.heads / a.pack) * a.batch;
     split_keys(a, vk::grad_keys(a.d), (columns + vk::kColumns - 1) / vk::kColumns * rest,
                a.d <= 64 ? Pace{2, 10, 1.6, 0.5} : Pace{2, 10, 1.1, 0.5}, 1);
+    if (a.rows) return;  // no gradient of the states
+    const int queries = vk::grad_queries(a.d), tiles = (a.tokens + queries - 1) / queries * (a.heads / a.kv_heads);
+    const int64_t slots = static_cast<int64_t>((a.length + vk::kSlot - 1) / vk::kSlot) * a.passages, per_block = vk::kColumns / vk::kSlot;
+    g.kv_splits = best_splits(tiles, 1, (slots + per_block - 1) / per_block * a.kv_heads * a.batch,
+                              a.d <= 64 ? Pace{2, 10, 1.4, 0.4} : Pace{1, 10, 1.25, 0}, 1,
+                              16.0 * a.batch * a.passages * a.length * a.kv_heads * a.d);
+    g.kv_tiles_per_split = (tiles + g.kv_splits - 1) / g.kv_splits;
 }
 size_t query_rows(const AttendArgs& a) { return static_cast<size_t>(a.batch) * a.heads * a.tokens; }
 size_t align(size_t x) { return (x + 15) / 16 * 16; }
+size_t part_bytes(const AttendArgs& a) { return a.splits == 1 ? 0 : align(a.splits * query_rows(a) * a.d * sizeof(float)); }
 size_t forward_bytes(const AttendArgs& a) {
-    return a.splits == 1 ? 0 : align(a.splits * query_rows(a) * a.d * sizeof(float)) + a.splits * query_rows(a) * sizeof(float2);
+    return a.splits == 1 ? 0 : part_bytes(a) + a.splits * query_rows(a) * sizeof(float2);
 }
 int table_parts(const AttendArgs& a) { return (a.tokens + vk::kColumns - 1) / vk::kColumns * a.batch * a.splits; }
 size_t table_bytes(const AttendArgs& a) {
     return a.bias.table ? align(static_cast<size_t>(table_parts(a)) * a.heads * a.bias.buckets * sizeof(float)) : 0;
 }
 size_t delta_bytes(const AttendArgs& a) { return align(query_rows(a) * sizeof(float)); }
-size_t backward_bytes(const AttendArgs& a) {
-    return delta_bytes(a) + table_bytes(a) + (a.splits == 1 ? 0 : a.splits * query_rows(a) * a.d * sizeof(float));
+size_t backward_bytes(const AttendGradArgs& g) {
+    const AttendArgs& a = g.a;
+    const size_t states = static_cast<size_t>(a.bank) * a.length * a.kv_heads;
+    return delta_bytes(a) + table_bytes(a) + part_bytes(a) + (g.kv_splits == 1 ? 0 : 2 * g.kv_splits * states * a.d * sizeof(float));
 }
 
 void check_workspace(void* workspace, size_t bytes, size_t needed) {
@@ -280,7 +292,7 @@ VK_EXPORT int vk_attend(const vk_attention* x, void* workspace, size_t workspace
         if (!query_rows(a)) return;
         if (a.splits > 1) {
             a.part = static_cast<float*>(workspace);
-            a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) + align(a.splits * query_rows(a) * a.d * sizeof(float)));
+            a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) + part_bytes(a));
         }
         const auto on = static_cast<hipStream_t>(stream);
         VK_HIP(few_columns(a) ? vk::launch_attend_few(a, x->type, on) : vk::launch_attend_forward(a, x->type, on));
@@ -291,9 +303,10 @@ VK_EXPORT int vk_attend(const vk_attention* x, void* workspace, size_t workspace
 VK_EXPORT int vk_attend_backward_workspace(const vk_attention* x, size_t* bytes) {
     return guarded([&] {
         valid(bytes != nullptr, "bytes is NULL");
-        AttendArgs a = args_of(x, false);
-        plan_backward(a);
-        *bytes = backward_bytes(a);
+        AttendGradArgs g;
+        g.a = args_of(x, false);
+        plan_backward(g);
+        *bytes = backward_bytes(g);
     });
 }
 
@@ -318,15 +331,16 @@ VK_EXPORT int vk_attend_backward(const vk_attention* x, const vk_attention_grad*
         valid(a.bias.table || !y->d_table, "d_table is given without a table");
         g.d_table = y->d_table;
         g.scale = x->scale;
-        plan_backward(a);
-        check_workspace(workspace, workspace_bytes, backward_bytes(a));
+        plan_backward(g);
+        check_workspace(workspace, workspace_bytes, backward_bytes(g));
         char* at = static_cast<char*>(workspace);
         g.delta = reinterpret_cast<float*>(at);
         g.table_part = reinterpret_cast<float*>(at + delta_bytes(a));
         a.part = reinterpret_cast<float*>(at + delta_bytes(a) + table_bytes(a));
+        g.kv_part = reinterpret_cast<float*>(at + delta_bytes(a) + table_bytes(a) + part_bytes(a));
         const auto on = static_cast<hipStream_t>(stream);
         if (query_rows(a)) VK_HIP(vk::launch_attend_grad_q(g, x->type, on));
         if (!x->rows && x->bank && x->length) VK_HIP(vk::launch_attend_grad_kv(g, x->type, on));
-        if (a.bias.table || (a.splits > 1 && query_rows(a))) VK_HIP(vk::launch_attend_grad_join(g, x->type, table_parts(a), on));
+        if (a.bias.table || (a.splits > 1 && query_rows(a)) || g.kv_splits > 1) VK_HIP(vk::launch_attend_grad_join(g, x->type, table_parts(a), on));
     });
 }

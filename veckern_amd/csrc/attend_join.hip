@@ -1,5 +1,5 @@
-// What follows the attention kernels where their work was split: the joined softmax of the splits of a row, the query
-// gradient's parts, and the bias table's gradient from the blocks' sums. All sum in a fixed order.
+// What follows the attention kernels where their work was split: the joined softmax of the splits of a row, the gradients'
+// parts, and the bias table's gradient from the blocks' sums. All sum in a fixed order.
 #include "attend_tile.hpp"
 
 namespace vk {
@@ -37,10 +37,10 @@ __global__ __launch_bounds__(256) void combine_kernel(AttendArgs a) {
     if (a.lse && e == 0) a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
 }
 
-// The first `query_blocks` blocks: d_q = scale * sum of the splits' parts, four elements a thread. The others: the table's
-// gradient, one wave per (bucket, head).
+// The first `query_blocks` blocks: d_q = scale * sum of the splits' parts, four elements a thread; the next `key_blocks`: d_k and
+// d_v alike. The others: the table's gradient, one wave per (bucket, head).
 template <class E>
-__global__ __launch_bounds__(256) void grad_join_kernel(AttendGradArgs g, int parts, int query_blocks) {
+__global__ __launch_bounds__(256) void grad_join_kernel(AttendGradArgs g, int parts, int query_blocks, int key_blocks) {
     const AttendArgs& a = g.a;
     if (static_cast<int>(blockIdx.x) < query_blocks) {
         const int groups = a.heads / a.pack, columns = a.tokens * a.pack, quads = a.d / 4;
@@ -60,7 +60,28 @@ __global__ __launch_bounds__(256) void grad_join_kernel(AttendGradArgs g, int pa
         *reinterpret_cast<u32x2*>(out) = *reinterpret_cast<u32x2*>(z);
         return;
     }
-    const int lane = threadIdx.x % 64, at = (blockIdx.x - query_blocks) * 4 + threadIdx.x / 64;
+    if (static_cast<int>(blockIdx.x) < query_blocks + key_blocks) {
+        const int quads = a.d / 4;
+        const int64_t states = a.bank * a.length * a.kv_heads, at = static_cast<int64_t>(blockIdx.x - query_blocks) * 256 + threadIdx.x;
+        if (at >= 2 * states * quads) return;
+        const bool value = at >= states * quads;
+        const int64_t state = at / quads - (value ? states : 0);
+        const int e = static_cast<int>(at % quads) * 4;
+        const float* part = g.kv_part + ((value ? g.kv_splits * states : 0) + state) * a.d + e;
+        f32x4 x{};
+#pragma unroll 4
+        for (int i = 0; i < g.kv_splits; ++i) x += *reinterpret_cast<const f32x4*>(part + i * states * a.d);
+        const int kv_head = state % a.kv_heads, key = state / a.kv_heads % a.length;
+        const int64_t row = state / a.kv_heads / a.length;
+        const AttendView& v = value ? g.d_v : g.d_k;
+        typename E::T z[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[j] = (typename E::T)(x[j] * (value ? 1.f : g.scale));
+        char* out = static_cast<char*>(v.p) + (row * v.outer + key * v.middle + kv_head * v.head + e) * 2;
+        *reinterpret_cast<u32x2*>(out) = *reinterpret_cast<u32x2*>(z);
+        return;
+    }
+    const int lane = threadIdx.x % 64, at = (blockIdx.x - query_blocks - key_blocks) * 4 + threadIdx.x / 64;
     if (at >= a.heads * a.bias.buckets) return;
     const int head = at % a.heads, bucket = at / a.heads;
     float x = 0.f;
@@ -83,10 +104,11 @@ hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stre
 hipError_t launch_attend_grad_join(const AttendGradArgs& g, int type, int parts, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t queries = a.splits > 1 ? (static_cast<int64_t>(a.batch) * a.heads * a.tokens * (a.d / 4) + 255) / 256 : 0;
-    const int64_t blocks = queries + (a.bias.table ? (static_cast<int64_t>(a.heads) * a.bias.buckets + 3) / 4 : 0);
+    const int64_t keys = g.kv_splits > 1 ? (2 * a.bank * a.length * a.kv_heads * (a.d / 4) + 255) / 256 : 0;
+    const int64_t blocks = queries + keys + (a.bias.table ? (static_cast<int64_t>(a.heads) * a.bias.buckets + 3) / 4 : 0);
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     auto kernel = type == kAttendBf16 ? attend::grad_join_kernel<attend::Bf16> : attend::grad_join_kernel<attend::F16>;
-    kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(g, parts, static_cast<int>(queries));
+    kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(g, parts, static_cast<int>(queries), static_cast<int>(keys));
     return hipGetLastError();
 }
 
