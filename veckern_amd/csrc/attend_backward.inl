@@ -5,7 +5,15 @@
 // Two kernels take 7 products where one would take 5, but each sums its own outputs in registers: no atomic sums in global
 // memory, no second copy of dQ in 32 bits, and the same bits from every run. P and dS are rounded to the inputs' type where
 // they become operands (the matrix instructions take 16 bits; in binary16 small dS need the loss scaling that training in
-// that type uses anyway); statistics, dP, delta and all sums are held in 32 bits.
+// that type uses anyway); statistics, dP, delta and all sums are held in 32 bits. delta is taken from the rounded output, as that
+// is what a program has kept: its error, of 2^-9 of the output's size in bfloat16, is the same for all keys of a row, and shows
+// most in the table's gradient, whose terms of a row cancel. Taking it from P dP instead would cost two more products.
+//
+// Measured: 32 requests of 512 tokens over their own, 12 heads of 64, a two-sided bias: queries 98 us, keys 83 us (390 and 620
+// TFLOP/s of the products done); 4 of 2048 tokens: 136 and 131 us. 2 of 2048 tokens over 4 x 2048, 16 heads of 128, no bias: 395 and
+// 635 us (1040 and 865 TFLOP/s). With heads of 64 the matrix cores are busy for 25 % and 35 % of the time, and the rest is VALU:
+// exponentials, bias and the table's sums; with 128 for 50 % and 39 %, LDS for 33 % and 37 %, and what is left are waits: of a tile
+// for its barrier, with two waves a SIMD, which registers limit.
 #include <type_traits>
 
 #include "attend_tile.hpp"
@@ -568,7 +576,9 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
 // wave's keys, values and two gradients would take more registers than two waves a SIMD may have:
 //   the first:  S = Q K^T, P = exp(...), dV += dO^T P, and P to LDS in 32 bits
 //   the second, one tile behind:  dP = dO V^T, dS = P (dP - delta), dK += Q^T dS
-// Both take as many products; three tiles lie in LDS, one for each of them and one to be filled.
+// Both take as many products; three tiles lie in LDS, one for each of them and one to be filled. (With a fourth tile and every
+// half's two products of different tiles, so that no product waits for its own tile's exponentials: 635 -> 700 us. 64 keys for two
+// waves of twice the registers: 673.)
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = grad_queries(DP);
@@ -780,10 +790,10 @@ hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch * g.kv_splits;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
-    if constexpr (DP <= 64) {  // two waves for 32 keys: 170 us where one takes 142 (4 x 2048 tokens, 12 heads of 64)
+    if constexpr (DP <= 64) {  // two waves for 32 keys: 170 us where one took 142 then (4 x 2048 tokens, 12 heads of 64)
         auto kernel = a.bias.table ? grad_kv_kernel<E, DP, true> : grad_kv_kernel<E, DP, false>;
         kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
-    } else {  // one wave for 32 keys: 767 us where two take 603 (2 x 2048 tokens over 4 x 2048 keys, 16 heads of 128)
+    } else {  // one wave for 32 keys: 767 us where two took 603 then (2 x 2048 tokens over 4 x 2048, 16 heads of 128)
         auto kernel = a.bias.table ? grad_kv_pair_kernel<E, DP, true> : grad_kv_pair_kernel<E, DP, false>;
         kernel<<<static_cast<unsigned>(blocks), 512, lds, stream>>>(g);
     }

@@ -9,6 +9,13 @@
 // normalises it, the maximum and the output are held in 32 bits. The weights are relative to a maximum that is only raised
 // when it grew by more than kSlack: the output's rescaling is rare, and P <= e^kSlack keeps its relative precision in either
 // type.
+//
+// Measured, and what bounds it (cards differ by 5 %): 4 requests of 512 tokens over 10 x 512 positions, 16 heads of 64: 62 us and
+// 7 for the join of three splits, 590 TFLOP/s. For each matrix instruction there are 10 others, two of them exponentials at a
+// quarter of the rate: the matrix cores are busy for 28 % of the time and the other instructions set the pace (more waves a
+// SIMD, which leaves each fewer registers, 77 us). 4096 tokens over 16 x 512, 16 heads of 128 over 4 key heads: 265 us,
+// 970 TFLOP/s; 4.7 others for a matrix instruction, matrix cores 45 %, LDS 34 %. 256 x 128 tokens with a bias, 12 heads of 64, the
+// keys of an encoder's own rows: 53 us for 164 MB, 3.1 TB/s: a block's two tiles are too few to hide its first loads.
 #include <type_traits>
 
 #include "attend_tile.hpp"
