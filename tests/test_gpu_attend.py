@@ -132,6 +132,16 @@ def test_many_tokens_over_few_states(shape, biased):
     both(q, k, v, lengths=lengths, d_out=d_out, **bias)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("length", [15, 40])
+def test_many_ragged_passages(d, length):
+    """Slots that hold a key are found over more passages than a wave has lanes, most of them empty in one request."""
+    batch, passages = 2, 150
+    q, k, v, _, lengths, d_out = make(d + length, BF16, batch, 20, passages, length, 4, 2, d, 0, True, empty=range(0, 130))
+    table = torch.randn(16, 4, generator=torch.Generator().manual_seed(d)).to(BF16).cuda()
+    both(q, k, v, lengths=lengths, d_out=d_out, table=table, buckets=16, max_distance=20, two_sided=True)
+
+
 @pytest.mark.parametrize("shape", [(2, 150, 5, 23, 4, 2, 32, 12, True), (3, 40, 9, 7, 2, 2, 16, 0, True),
                                    (1, 300, 1, 190, 2, 1, 24, 0, False)], ids=str)
 def test_small_heads(shape):

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
     const int columns = a.tokens * a.pack, column_tiles = (columns + kColumns - 1) / kColumns, groups = a.heads / a.pack;
-    int place = xcd_place(blockIdx.x, gridDim.x);
+    int place = xcd_place(blockIdx.x, gridDim.x, column_tiles * a.splits);
     const int column_tile = place % column_tiles;
     place /= column_tiles;
     const int split = place % a.splits;
@@ -341,20 +341,60 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     }
 }
 
-// Writes a key's d_k or d_v, or a split's part of it. Keys past the row's length have no gradient: zeros.
+// Keys come in slots of 16 positions of a passage. A block takes eight of a request's slots that hold a key, in order, so that what
+// ragged passages leave empty costs no products; and beside them it writes the zeros of the keys that are absent in the eight slots
+// that would be its own if all were full. (8 requests of 256 tokens over 8 passages of up to 256 positions, 8 key heads of 128: 108 us
+// with a block's own slots whatever they held, 94 so; 33 of 84 over 14 of up to 511: 161 and 136; blocks of one tile pay for the
+// search, 217 of 27 over 4 of up to 48: 95 and 102.)
+struct KeySlot {
+    int row, first, left;
+};
+// The lane's of the wave's two slots, `slot` and the next. All lanes of the wave call it.
+__device__ __forceinline__ KeySlot key_slot(const AttendArgs& a, int b, int slot, int per_row, int lane) {
+    if (!a.lengths) {
+        const int own = slot + lane % 32 / kSlot, passage = own / per_row, first = (own - passage * per_row) * kSlot;
+        return passage < a.passages ? KeySlot{b * a.passages + passage, first, a.length - first} : KeySlot{0, 0, 0};
+    }
+    KeySlot x[2] = {};
+    int before = 0, found = 0;
+    for (int r0 = 0; r0 < a.passages && found < 2; r0 += 64) {
+        const int count = r0 + lane < a.passages ? min(max(a.lengths[b * a.passages + r0 + lane], 0), a.length) : 0;
+        const int slots = (count + kSlot - 1) / kSlot;
+        const int upto = wave_sums(slots);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint64_t at = __ballot(before + upto > slot + i);
+            if (found > i || !at) continue;
+            const int l = __builtin_ctzll(at), n = slot + i - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(slots, l));
+            x[i] = {b * a.passages + r0 + l, n * kSlot, __builtin_amdgcn_readlane(count, l) - n * kSlot};
+            found = i + 1;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (found < 2) x[1].first = x[0].first;  // what is not there lies beside what is
+    return lane % 32 < kSlot ? x[0] : x[1];
+}
+// Row and position of the lane's key in the slots as they would be if all were full, where it is past the row's length; else (0, -1).
+__device__ __forceinline__ int2 absent_key(const AttendArgs& a, int b, int slot, int per_row, int lane) {
+    const int own = slot + lane % 32 / kSlot, passage = own / per_row, key = (own - passage * per_row) * kSlot + lane % kSlot;
+    if (!a.lengths || passage >= a.passages || key >= a.length) return make_int2(0, -1);
+    const int row = b * a.passages + passage;
+    return key < a.lengths[row] ? make_int2(0, -1) : make_int2(row, key);
+}
+
+// Writes a key's d_k or d_v, or a split's part of it.
 template <class E, int DP>
-__device__ __forceinline__ void store_key(const AttendGradArgs& g, bool value, int split, int row, int key, int kv_head, int hi, bool there,
+__device__ __forceinline__ void store_key(const AttendGradArgs& g, bool value, int split, int row, int key, int kv_head, int hi,
                                           const f32x16 (&sum)[DP / 32]) {
     const AttendArgs& a = g.a;
     const AttendView& v = value ? g.d_v : g.d_k;
-    const f32x16 zero{};
     auto each = [&](auto&& store) {
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
                 const int e = 32 * i + mfma_row(4 * quad, hi);
-                if (e < a.d) store(e, there ? sum[i] : zero, quad);
+                if (e < a.d) store(e, sum[i], quad);
             }
     };
     if (g.kv_splits > 1) {
@@ -383,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
     const int share = a.heads / a.kv_heads, per_row = (a.length + kSlot - 1) / kSlot;
     const int key_tiles = (per_row * a.passages + kColumns / kSlot - 1) / (kColumns / kSlot);
-    int place = xcd_place(blockIdx.x, gridDim.x);
+    int place = xcd_place(blockIdx.x, gridDim.x, key_tiles * g.kv_splits);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
     int split = 0;
@@ -392,12 +432,16 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         place /= g.kv_splits;
     }
     const int kv_head = place % a.kv_heads, b = place / a.kv_heads;
-    // the lane's key, by slots: of the passages of a request, 16 positions each
-    const int slot = key_tile * (kColumns / kSlot) + wave * 2 + lane % 32 / kSlot, passage = slot / per_row;
-    const int first_key = (slot - passage * per_row) * kSlot, key = first_key + lane % kSlot;
-    const bool inside = passage < a.passages;
-    const int row = b * a.passages + (inside ? passage : 0);
-    const bool there = inside && key < (a.lengths ? min(a.lengths[row], a.length) : a.length);
+    const int slot = key_tile * (kColumns / kSlot) + wave * 2;
+    const KeySlot mine = key_slot(a, b, slot, per_row, lane);
+    const int row = mine.row, first_key = mine.first, key = first_key + lane % kSlot;
+    const bool there = lane % kSlot < mine.left;
+    const int2 absent = absent_key(a, b, slot, per_row, lane);
+    if (absent.y >= 0) {
+        const f32x16 none[kParts] = {};
+        store_key<E, DP>(g, false, split, absent.x, absent.y, kv_head, hi, none);
+        store_key<E, DP>(g, true, split, absent.x, absent.y, kv_head, hi, none);
+    }
 
     f32x16 dk[kParts], dv[kParts];
 #pragma unroll
@@ -566,9 +610,9 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         else run(std::false_type());
     }
 
-    if (inside && key < a.length) {
-        store_key<E, DP>(g, false, split, row, key, kv_head, hi, there, dk);
-        store_key<E, DP>(g, true, split, row, key, kv_head, hi, there, dv);
+    if (there) {
+        store_key<E, DP>(g, false, split, row, key, kv_head, hi, dk);
+        store_key<E, DP>(g, true, split, row, key, kv_head, hi, dv);
     }
 }
 
@@ -594,7 +638,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
     const bool second = uniform(thread / 256) != 0;
     const int share = a.heads / a.kv_heads, per_row = (a.length + kSlot - 1) / kSlot;
     const int key_tiles = (per_row * a.passages + kColumns / kSlot - 1) / (kColumns / kSlot);
-    int place = xcd_place(blockIdx.x, gridDim.x);
+    int place = xcd_place(blockIdx.x, gridDim.x, key_tiles * g.kv_splits);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
     int split = 0;
@@ -603,12 +647,15 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         place /= g.kv_splits;
     }
     const int kv_head = place % a.kv_heads, b = place / a.kv_heads;
-    // the lane's key, by slots: of the passages of a request, 16 positions each
-    const int slot = key_tile * (kColumns / kSlot) + wave * 2 + lane % 32 / kSlot, passage = slot / per_row;
-    const int first_key = (slot - passage * per_row) * kSlot, key = first_key + lane % kSlot;
-    const bool inside = passage < a.passages;
-    const int row = b * a.passages + (inside ? passage : 0);
-    const bool there = inside && key < (a.lengths ? min(a.lengths[row], a.length) : a.length);
+    const int slot = key_tile * (kColumns / kSlot) + wave * 2;
+    const KeySlot mine = key_slot(a, b, slot, per_row, lane);
+    const int row = mine.row, first_key = mine.first, key = first_key + lane % kSlot;
+    const bool there = lane % kSlot < mine.left;
+    const int2 absent = absent_key(a, b, slot, per_row, lane);
+    if (absent.y >= 0) {
+        const f32x16 none[kParts] = {};
+        store_key<E, DP>(g, !second, split, absent.x, absent.y, kv_head, hi, none);
+    }
 
     f32x16 sum[kParts];  // dV or dK
 #pragma unroll
@@ -763,7 +810,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
         else both(std::false_type());
     }
 
-    if (inside && key < a.length) store_key<E, DP>(g, !second, split, row, key, kv_head, hi, there, sum);
+    if (there) store_key<E, DP>(g, !second, split, row, key, kv_head, hi, sum);
 }
 
 template <class E, int DP>

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(A
     extern __shared__ __align__(16) char shared[];  // tiles of each wave; (row, positions) of the passages; the bias by distance
     const int thread = threadIdx.x, lane = thread % 64, wave = uniform(thread / 64), hi = lane / 32;
     const int columns = a.tokens * a.pack, column_tiles = (columns + 31) / 32, groups = a.heads / a.pack;
-    int place = xcd_place(blockIdx.x, gridDim.x);
+    int place = xcd_place(blockIdx.x, gridDim.x, column_tiles * a.splits);
     const int column_tile = place % column_tiles;
     place /= column_tiles;
     const int split = place % a.splits;

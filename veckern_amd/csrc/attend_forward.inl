@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
     const int columns = a.tokens * a.pack, column_tiles = (columns + kColumns - 1) / kColumns, groups = a.heads / a.pack;
-    int place = xcd_place(blockIdx.x, gridDim.x);
+    int place = xcd_place(blockIdx.x, gridDim.x, column_tiles * a.splits);
     const int column_tile = place % column_tiles;
     place /= column_tiles;
     const int split = place % a.splits;

@@ -64,6 +64,17 @@ __device__ __forceinline__ float wave_sum(float x) {
     return x;
 }
 
+// A lane's and all lower lanes' sum.
+__device__ __forceinline__ int wave_sums(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // one, two, four, eight lanes up within 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of the first and third 16 to the next
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+    return x;
+}
+
 // Tiles in LDS: rows of DP 16-bit elements, 16 bytes apart. A ds_read_b128 of 16 consecutive lanes takes 16 bytes of 16 rows,
 // the transposing read of 32 lanes 64 bytes of rows that are four apart: either covers the 64 banks of 4 bytes once. Every
 // place of a tile is one lane's address plus a constant, so the reads take two address registers in all.
@@ -302,11 +313,21 @@ __device__ __forceinline__ int2 reach(const Slot (&s)[SLOTS]) {
     return make_int2(x.x, x.y + kSlot - 1);
 }
 
-// Blocks that read the same keys follow each other in the order of `place`; the hardware deals block ids over the 8 XCDs in
-// turn, so each XCD is given one run of places and its L2 sees the same keys again.
-__device__ __forceinline__ int xcd_place(int id, int total) {
-    const int q = total / 8, extra = total % 8, x = id % 8, i = id / 8;
-    return x * q + min(x, extra) + i;
+// Blocks that read the same keys (or queries) follow each other in the order of places, `each` to a group. The hardware deals
+// block ids over the 8 XCDs in turn: two groups that follow each other, of neighbouring heads as a rule, go to one XCD, whose L2
+// sees what they read again, and the pairs to the XCDs in turn, so that ragged requests load them alike; what is left over is cut
+// into 8 runs. (9 requests of up to 1592 tokens over their own, 12 heads of 64: 103, 168 and 168 us for the forward pass, the
+// queries' and the keys' gradient where all groups were cut into 8 runs, 96, 147 and 137 so; 32 of 512 each take the same time.)
+__device__ __forceinline__ int xcd_place(int id, int total, int each) {
+    each *= 2;
+    const int whole = total / each / 8 * 8 * each;
+    if (id < whole) {
+        const int i = id / 8, group = i / each;
+        return (group * 8 + id % 8) * each + (i - group * each);
+    }
+    id -= whole;
+    const int q = (total - whole) / 8, extra = (total - whole) % 8, x = id % 8, i = id / 8;
+    return whole + x * q + min(x, extra) + i;
 }
 
 // The bias by distance in LDS: held[i] = table[bucket(i - far - kPad)][head], i in [0, 2 * far + 2 * kPad]. Every distance from
