@@ -9,74 +9,47 @@
 // is what a program has kept: its error, of 2^-9 of the output's size in bfloat16, is the same for all keys of a row, and shows
 // most in the table's gradient, whose terms of a row cancel. Taking it from P dP instead would cost two more products.
 //
-// Measured: 32 requests of 512 tokens over their own, 12 heads of 64, a two-sided bias: queries 98 us, keys 83 us (390 and 620
-// TFLOP/s of the products done); 4 of 2048 tokens: 136 and 131 us. 2 of 2048 tokens over 4 x 2048, 16 heads of 128, no bias: 395 and
-// 635 us (1040 and 865 TFLOP/s). With heads of 64 the matrix cores are busy for 25 % and 35 % of the time, and the rest is VALU:
+// Measured: 32 requests of 512 tokens over their own, 12 heads of 64, a two-sided bias: queries 93 us, keys 77 us (415 and 670
+// TFLOP/s of the products done), of which 30 and 14 us go by where no key is there: the reading of a block's own columns and
+// the writing of its results, which all blocks do at about the same time; 4 of 2048 tokens: 135 and 131 us. 2 of 2048 tokens over
+// 4 x 2048, 16 heads of 128, no bias: 395 and 610 us (1040 and 900 TFLOP/s). With heads of 64 the matrix cores are busy for 25 % and 35 % of the time, and the rest is VALU:
 // exponentials, bias and the table's sums; with 128 for 50 % and 39 %, LDS for 33 % and 37 %, and what is left are waits: of a tile
 // for its barrier, with two waves a SIMD, which registers limit.
-#include <type_traits>
-
 #include "attend_tile.hpp"
 
 namespace vk::attend {
 
-template <class T>
-__device__ __forceinline__ void store_four(void* p, int at, const f32x16& x, int quad, float factor) {
-    T y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = (T)(x[4 * quad + j] * factor);
-    *reinterpret_cast<u32x2*>(static_cast<char*>(p) + at * 2) = *reinterpret_cast<u32x2*>(y);
-}
-
 // Adds dS of a 32 x 32 tile (lane: one query position, x: the distance of the tile's first key from the first query) to a
-// wave's sums by distance, in a fixed order, in one of two ways; past the ends of the buckets a sum goes to a register. (An LDS
-// atomic for each element took 130 clocks an instruction.)
-//   skewed: the tile goes through LDS by diagonals, element (key, query) to row 31 + key - query and place `query` of `skew`,
-//     whose other places stay zero; then a lane sums one diagonal. With 36 floats a row neither the writes nor the 16-byte reads
-//     share a bank.
-//   turned: of each result, rows n and n + 1 in the two halves of the wave, the queries are turned by n lanes within a half:
-//     then lane j has the distances -j and 32 - j of every row (one more in the upper half), and adds what it is given to one of
-//     two sums.
-// The first takes fewer instructions (32 requests of 512 tokens, 64 elements, far 91: 99 us against 110), but 36 KB a block: where
-// two blocks of a compute unit then have no room, the second is faster (26 requests of 714 tokens and 162 keys, far 469: 104 us
-// against 76).
-constexpr int kSkew = 36, kSkewFloats = 63 * kSkew;
-template <int R>
-__device__ __forceinline__ void turn(const f32x16& ds, int lane, float& near, float& further) {
-    constexpr int n = tile_row(R, 0), kTurn = 0xc000 | n << 5;  // lane j of 32 reads lane (j + n) % 32
-    const float x = n ? __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(ds[R]), kTurn)) : ds[R];
-    const bool turned = lane % 32 >= 32 - n;
-    near += turned ? 0.f : x;
-    if (n) further += turned ? x : 0.f;
-    if constexpr (R < 15) turn<R + 1>(ds, lane, near, further);
+// wave's sums by distance, in a fixed order. Of each result, rows n and n + 1 in the two halves of the wave, the queries are turned
+// by n lanes within a half: then lane j has the distances -j and 32 - j of every row (one more in the upper half), and adds what it
+// is given to one of two sums. Past the ends of the buckets a sum goes to a register. (An LDS atomic for each element took 130
+// clocks an instruction. Diagonals summed through a skewed tile in LDS took the same time, but 9 KB a wave: from far = 147 on only
+// one block then had room on a compute unit, and 26 requests of 714 tokens and 162 keys, far 469, took 104 us where this takes 66.)
+template <int FROM, int... R>
+__device__ __forceinline__ void turn(const f32x16& ds, float (&x)[8], std::integer_sequence<int, R...>) {
+    // lane j of 32 reads lane (j + n) % 32, n = tile_row(r, 0)
+    ((x[R] = __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(ds[FROM + R]), 0xc000 | tile_row(FROM + R, 0) << 5))), ...);
 }
-template <bool SKEWED>
-__device__ __forceinline__ void add_diagonals(const f32x16& ds, float* skew, float* sums, int far, int x, int lane, float& below, float& above) {
-    float sum;
-    int distance;
-    if constexpr (SKEWED) {
-        float* to = skew + (31 - lane % 32 + lane / 32) * kSkew + lane % 32;
+__device__ __forceinline__ void add_diagonals(const f32x16& ds, float* sums, int far, int x, int lane, float& below, float& above) {
+    float near = 0.f, further = 0.f;  // distance -j and 32 - j
+    float turned[2][8];  // eight under way while eight are added
+    turn<0>(ds, turned[0], std::make_integer_sequence<int, 8>());
+    between_runs();
+    turn<8>(ds, turned[1], std::make_integer_sequence<int, 8>());
+    between_runs();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) to[tile_row(r, 0) * kSkew] = ds[r];
-        between_lanes();
-        const f32x4* from = reinterpret_cast<const f32x4*>(skew + min(lane, 62) * kSkew);
-        f32x4 y = from[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) y += from[i];
-        sum = lane < 63 ? (y[0] + y[1]) + (y[2] + y[3]) : 0.f;
-        distance = x + lane - 31;
-    } else {
-        float near = 0.f, further = 0.f;  // distance -j and 32 - j
-        turn<0>(ds, lane, near, further);
-        // both sums of the lower half, and beside them those of the upper half, which belong to the lane before
-        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(near), __float_as_uint(further), false, false);
-        sum = __uint_as_float(y[0]) + __int_as_float(__builtin_amdgcn_ds_bpermute((lane + 1) % 64 * 4, y[1]));
-        distance = x - lane % 32 + (lane & 32);
+    for (int r = 0; r < 16; ++r) {
+        const bool over = lane % 32 >= 32 - tile_row(r, 0);
+        near += over ? 0.f : turned[r / 8][r % 8];
+        further += over ? turned[r / 8][r % 8] : 0.f;
     }
-    const int place = distance + far + kPad;
+    // both sums of the lower half, and beside them those of the upper half, which belong to the lane before
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(near), __float_as_uint(further), false, false);
+    const float sum = __uint_as_float(y[0]) + __int_as_float(__builtin_amdgcn_ds_bpermute((lane + 1) % 64 * 4, y[1]));
+    const int place = x - lane % 32 + (lane & 32) + far + kPad;
     if (place < 0) below += sum;
     else if (place > 2 * far + 2 * kPad) above += sum;
-    else if (!SKEWED || lane < 63) sums[place] += sum;
+    else sums[place] += sum;
     between_lanes();
 }
 
@@ -86,18 +59,15 @@ __device__ __forceinline__ int bucket_begin(const AttendBias& s, int j) {
     return j <= exact ? j : j - exact - 1 < s.edges ? s.edge[j - exact - 1] : s.far + kPad + 1;
 }
 
-// How the table's gradient is summed, if there is one.
-enum TableSums { kNoTable, kSkewedSums, kTurnedSums };
-
-template <class E, int DP, TableSums SUMS>
-__global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
+// With 32 elements a head three waves a SIMD: 32 requests of 512 tokens, 12 heads, 66 us where two take 78.
+template <class E, int DP, bool BIAS>
+__global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGradArgs g) {
     // with 128 elements a head two waves a SIMD have no registers for more
-    constexpr bool BIAS = SUMS != kNoTable, kSkewed = SUMS == kSkewedSums;
     constexpr int kSteps = DP / 16, kParts = DP / 32, kKeys = grad_keys(DP), kSubs = kKeys / 32, kSlots = kKeys / kSlot;
     const AttendArgs& a = g.a;
     __shared__ __align__(16) char tile[2][2][kTileBytes<DP, kKeys>];
     __shared__ int2 found[kHeldPassages];
-    extern __shared__ float shared[];  // per wave a skewed tile; the bias by distance; per wave its gradient's sums by distance
+    extern __shared__ float held[];  // the bias by distance; per wave its gradient's sums by distance
 
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
     const int columns = a.tokens * a.pack, column_tiles = (columns + kColumns - 1) / kColumns, groups = a.heads / a.pack;
@@ -116,11 +86,11 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     auto at = [&](const AttendView& v) { return b * v.outer + token * v.middle + head * v.head; };
     s16x8 qf[kSteps], df[kSteps], of[kSteps];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        qf[i] = column(a.q, at(a.q), used, i, hi, a.d);
-        df[i] = column(g.d_out, at(g.d_out), used, i, hi, a.d);
-        of[i] = column(a.out, at(a.out), used, i, hi, a.d);
-    }
+    for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, at(a.q), used, i, hi, a.d);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) df[i] = column(g.d_out, at(g.d_out), used, i, hi, a.d);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) of[i] = column(a.out, at(a.out), used, i, hi, a.d);
     float2 lse = used ? a.lse[row] : make_float2(-INFINITY, 0.f);
     const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
     places.fill(a, b, found, thread, 256);
@@ -140,15 +110,11 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     int position = 0;
     float below = 0.f, above = 0.f;
     bool large = false;
-    float *held = nullptr, *sums = nullptr, *skew = nullptr;
+    float* sums = nullptr;
     if constexpr (BIAS) {
         const int distances = bias_places(a.bias.far);
-        skew = shared + wave * kSkewFloats;
-        held = shared + (kSkewed ? 4 * kSkewFloats : 0);
         sums = held + (1 + wave) * distances;
         large = fill_biases<E>(a.bias, head, 1, a.scale, held, thread, 256);
-        if constexpr (kSkewed)
-            for (int i = thread; i < 4 * kSkewFloats; i += 256) shared[i] = 0.f;
         for (int i = thread; i < 4 * distances; i += 256) held[distances + i] = 0.f;
         position = token + a.q_start_all + (a.q_start ? a.q_start[b] : 0);
     }
@@ -171,26 +137,24 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     }
     __syncthreads();
     const char *k, *v;
-    auto products = [&](f32x16 (&s)[kSubs], f32x16 (&dp)[kSubs]) {
-#pragma unroll
-        for (int sub = 0; sub < kSubs; ++sub) {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                if (i) s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
-                dp[sub] = E::mfma(straight<DP>(v, 32 * sub, i, lane), df[i], dp[sub]);
-            }
-        }
+    // all but the first of a sub-tile's logits: dP's first step, and the others of both in turn
+    auto logits = [&](f32x16 (&s)[kSubs], f32x16 (&dp)[kSubs]) {
+        constexpr int kEach = 2 * kSteps - 1;
+        products<kSubs * kEach, 1, 4>(
+            [&](int i) { return straight<DP>(i % kEach % 2 ? k : v, 32 * (i / kEach), (i % kEach + 1) / 2, lane); },
+            [&](int i, s16x8 x) {
+                const int sub = i / kEach, step = (i % kEach + 1) / 2;
+                if (i % kEach % 2) s[sub] = E::mfma(x, qf[step], s[sub]);
+                else dp[sub] = E::mfma(x, df[step], dp[sub]);
+            });
     };
     auto gather = [&](const f32x16& ds, int sub) {
-        between_runs();
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const s16x8 x = rounded<E>(ds, half);
-#pragma unroll
-            for (int i = 0; i < kParts; ++i) dq[i] = E::mfma(transposed<DP>(k, 32 * sub + 16 * half, i, lane), x, dq[i]);
-        }
-        feed<2 * kParts, 2, 3>();
-        between_runs();
+        s16x8 y;
+        products<2 * kParts, 2, 3>([&](int i) { return transposed<DP>(k, 32 * sub + 16 * (i / kParts), i % kParts, lane); },
+                                   [&](int i, s16x8 x) {
+                                       if (i % kParts == 0) y = rounded<E>(ds, i / kParts);
+                                       dq[i % kParts] = E::mfma(x, y, dq[i % kParts]);
+                                   });
     };
     auto run = [&](auto kind) {
         constexpr bool kLarge = decltype(kind)::value;
@@ -225,10 +189,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
 #pragma unroll
                 for (int sub = 0; sub < kSubs; ++sub) s[sub] = E::mfma(straight<DP>(k, 32 * sub, 0, lane), qf[0], f32x16{});
             }
-            between_runs();
-            products(s, dp);
-            feed<2 * kSubs * kSteps - kSubs, 1, 4>();
-            between_runs();
+            logits(s, dp);
             if constexpr (kLarge) {
 #pragma unroll
                 for (int sub = 0; sub < kSubs; ++sub)
@@ -257,13 +218,13 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
                             f32x16 one = s[sub];
 #pragma unroll
                             for (int r = 0; r < 8; ++r) one[r] = 0.f;
-                            add_diagonals<kSkewed>(one, skew, sums, a.bias.far, y.first - kSlot - t0, lane, below, above);
+                            add_diagonals(one, sums, a.bias.far, y.first - kSlot - t0, lane, below, above);
                             one = s[sub];
 #pragma unroll
                             for (int r = 8; r < 16; ++r) one[r] = 0.f;
-                            add_diagonals<kSkewed>(one, skew, sums, a.bias.far, x.first - t0, lane, below, above);
+                            add_diagonals(one, sums, a.bias.far, x.first - t0, lane, below, above);
                         } else {
-                            add_diagonals<kSkewed>(s[sub], skew, sums, a.bias.far, x.first - t0, lane, below, above);
+                            add_diagonals(s[sub], sums, a.bias.far, x.first - t0, lane, below, above);
                         }
                     }
                 } else {
@@ -300,12 +261,7 @@ __global__ __launch_bounds__(256, 2) void grad_q_kernel(AttendGradArgs g) {
     } else if (used) {
         char* out = static_cast<char*>(g.d_q.p) + at(g.d_q) * 2;
 #pragma unroll
-        for (int i = 0; i < kParts; ++i)
-#pragma unroll
-            for (int quad = 0; quad < 4; ++quad) {
-                const int e = 32 * i + mfma_row(4 * quad, hi);
-                if (e < a.d) store_four<typename E::T>(out, e, dq[i], quad, g.scale);
-            }
+        for (int i = 0; i < kParts; ++i) store_column<E>(out, dq[i], i, hi, a.d, g.scale);
     }
     if constexpr (BIAS) {
         const AttendBias& s = a.bias;
@@ -388,24 +344,20 @@ __device__ __forceinline__ void store_key(const AttendGradArgs& g, bool value, i
                                           const f32x16 (&sum)[DP / 32]) {
     const AttendArgs& a = g.a;
     const AttendView& v = value ? g.d_v : g.d_k;
-    auto each = [&](auto&& store) {
+    if (g.kv_splits > 1) {
+        float* part = g.kv_part + ((((value ? g.kv_splits : 0) + split) * a.bank + row) * a.length + key) * a.kv_heads * a.d + kv_head * a.d;
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
             for (int quad = 0; quad < 4; ++quad) {
                 const int e = 32 * i + mfma_row(4 * quad, hi);
-                if (e < a.d) store(e, sum[i], quad);
+                if (e < a.d)
+                    *reinterpret_cast<f32x4*>(part + e) = f32x4{sum[i][4 * quad], sum[i][4 * quad + 1], sum[i][4 * quad + 2], sum[i][4 * quad + 3]};
             }
-    };
-    if (g.kv_splits > 1) {
-        float* part = g.kv_part + ((((value ? g.kv_splits : 0) + split) * a.bank + row) * a.length + key) * a.kv_heads * a.d + kv_head * a.d;
-        each([&](int e, const f32x16& x, int quad) {
-            *reinterpret_cast<f32x4*>(part + e) = f32x4{x[4 * quad], x[4 * quad + 1], x[4 * quad + 2], x[4 * quad + 3]};
-        });
     } else {
         char* out = static_cast<char*>(v.p) + (row * v.outer + key * v.middle + kv_head * v.head) * 2;
-        const float factor = value ? 1.f : g.scale;
-        each([&](int e, const f32x16& x, int quad) { store_four<typename E::T>(out, e, x, quad, factor); });
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) store_column<E>(out, sum[i], i, hi, a.d, value ? 1.f : g.scale);
     }
 }
 
@@ -491,10 +443,9 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
             const int64_t k = row * a.k.outer + key * a.k.middle + kv_head * a.k.head;
             const int64_t v = row * a.v.outer + key * a.v.middle + kv_head * a.v.head;
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                kf[i] = column(a.k, k, there, i, hi, a.d);
-                vf[i] = column(a.v, v, there, i, hi, a.d);
-            }
+            for (int i = 0; i < kSteps; ++i) kf[i] = column(a.k, k, there, i, hi, a.d);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) vf[i] = column(a.v, v, there, i, hi, a.d);
         }
         bool large = false;
         if constexpr (BIAS) {
@@ -510,26 +461,26 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
         auto of = [&](int which, int sub, int quad) {
             return *reinterpret_cast<const f32x4*>(&stat[now][which][32 * sub + mfma_row(4 * quad, hi)]);
         };
-        auto products = [&](f32x16 (&s)[2], f32x16 (&dp)[2]) {
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    s[sub] = E::mfma(straight<DP>(q, 32 * sub, i, lane), kf[i], s[sub]);
-                    dp[sub] = E::mfma(straight<DP>(d, 32 * sub, i, lane), vf[i], dp[sub]);
-                }
-            }
+        auto logits = [&](f32x16 (&s)[2], f32x16 (&dp)[2]) {
+            products<4 * kSteps, 1, 4>([&](int i) { return straight<DP>(i % 2 ? d : q, 32 * (i / (2 * kSteps)), i / 2 % kSteps, lane); },
+                                       [&](int i, s16x8 x) {
+                                           const int sub = i / (2 * kSteps), step = i / 2 % kSteps;
+                                           if (i % 2) dp[sub] = E::mfma(x, vf[step], dp[sub]);
+                                           else s[sub] = E::mfma(x, kf[step], s[sub]);
+                                       });
         };
         auto gather = [&](const f32x16 (&p)[2], const f32x16 (&ds)[2]) {
-#pragma unroll
-            for (int half = 0; half < 4; ++half) {
-                const s16x8 x = rounded<E>(p[half / 2], half % 2), y = rounded<E>(ds[half / 2], half % 2);
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) {
-                    dv[i] = E::mfma(transposed<DP>(d, 16 * half, i, lane), x, dv[i]);
-                    dk[i] = E::mfma(transposed<DP>(q, 16 * half, i, lane), y, dk[i]);
-                }
-            }
+            s16x8 y, z;
+            products<8 * kParts, 2, 3>([&](int i) { return transposed<DP>(i % 2 ? q : d, 16 * (i / (2 * kParts)), i / 2 % kParts, lane); },
+                                       [&](int i, s16x8 x) {
+                                           const int half = i / (2 * kParts), part = i / 2 % kParts;
+                                           if (i % (2 * kParts) == 0) {
+                                               y = rounded<E>(p[half / 2], half % 2);
+                                               z = rounded<E>(ds[half / 2], half % 2);
+                                           }
+                                           if (i % 2) dk[part] = E::mfma(x, z, dk[part]);
+                                           else dv[part] = E::mfma(x, y, dv[part]);
+                                       });
         };
         auto run = [&](auto kind) {
             constexpr bool kLarge = decltype(kind)::value;
@@ -568,10 +519,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                                           [&](int r, float x) { s[sub][r] += x; });
                     }
                 }
-                between_runs();
-                products(s, dp);
-                feed<4 * kSteps, 1, 4>();
-                between_runs();
+                logits(s, dp);
                 if constexpr (kLarge) {
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub) {
@@ -591,10 +539,7 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
                     s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]);
                     dp[r / 16][r % 16] *= s[r / 16][r % 16];
                 }
-                between_runs();
                 gather(s, dp);
-                feed<8 * kParts, 2, 3>();
-                between_runs();
                 if (more) store(now ^ 1);
                 if constexpr (BIAS) {
                     if (turned && more) {  // another head's bias, once every wave is done with this one's
@@ -621,8 +566,8 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
 //   the first:  S = Q K^T, P = exp(...), dV += dO^T P, and P to LDS in 32 bits
 //   the second, one tile behind:  dP = dO V^T, dS = P (dP - delta), dK += Q^T dS
 // Both take as many products; three tiles lie in LDS, one for each of them and one to be filled. (With a fourth tile and every
-// half's two products of different tiles, so that no product waits for its own tile's exponentials: 635 -> 700 us. 64 keys for two
-// waves of twice the registers: 673.)
+// half's two products of different tiles, so that no product waits for its own tile's exponentials: 635 -> 700 us then. 64 keys
+// for two waves of twice the registers: 673.)
 template <class E, int DP, bool BIAS>
 __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) {
     constexpr int kSteps = DP / 16, kParts = DP / 32, kQueries = grad_queries(DP);
@@ -693,23 +638,17 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                 stat[to][3][at] = low;
             }
         };
-        auto products = [&](f32x16 s, const char* rows) {
-            between_runs();
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) s = E::mfma(straight<DP>(rows, 0, i, lane), own[i], s);
-            feed<kSteps, 1, 4>();
-            between_runs();
+        auto logits = [&](f32x16 s, const char* rows) {
+            products<kSteps, 1, 4>([&](int i) { return straight<DP>(rows, 0, i, lane); }, [&](int i, s16x8 x) { s = E::mfma(x, own[i], s); });
             return s;
         };
-        auto gather = [&](const f32x16& x, const char* rows) {
-            between_runs();
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const s16x8 y = rounded<E>(x, half);
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) sum[i] = E::mfma(transposed<DP>(rows, 16 * half, i, lane), y, sum[i]);
-            }
-            feed<2 * kParts, 2, 3>();
+        auto gather = [&](const f32x16& z, const char* rows) {
+            s16x8 y;
+            products<2 * kParts, 2, 3>([&](int i) { return transposed<DP>(rows, 16 * (i / kParts), i % kParts, lane); },
+                                       [&](int i, s16x8 x) {
+                                           if (i % kParts == 0) y = rounded<E>(z, i / kParts);
+                                           sum[i % kParts] = E::mfma(x, y, sum[i % kParts]);
+                                       });
         };
         int head = kv_head * share, first = 0;  // of the tile that is loaded next
         if (split) {
@@ -763,7 +702,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                             each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), key - (from + start + 16 + hi), [&](int r, float x) { s[r] += x; });
                         }
                     }
-                    s = products(s, tile[now][0]);
+                    s = logits(s, tile[now][0]);
                     if constexpr (kLarge) {
                         const f32x16 l = begin(now, 2), low = begin(now, 3);
                         each_bias<-1>(bias_held, a.bias.far, key - (from + start + hi), key - (from + start + 16 + hi), [&](int r, float x) {
@@ -780,7 +719,7 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
                         handed[n % 2][wave][quad][lane] = f32x4{s[4 * quad], s[4 * quad + 1], s[4 * quad + 2], s[4 * quad + 3]};
                     gather(s, tile[now][1]);
                 } else if (kSecond && n > 0) {
-                    f32x16 dp = products(begin(before, 1), tile[before][1]);
+                    f32x16 dp = logits(begin(before, 1), tile[before][1]);
 #pragma unroll
                     for (int quad = 0; quad < 4; ++quad) {
                         const f32x4 p = handed[(n + 1) % 2][wave][quad][lane];
@@ -818,14 +757,8 @@ hipError_t launch_grad_q(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns * (a.heads / a.pack) * a.batch * a.splits;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-    size_t lds = a.bias.table ? 5 * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
-    auto kernel = a.bias.table ? grad_q_kernel<E, DP, kTurnedSums> : grad_q_kernel<E, DP, kNoTable>;
-    constexpr size_t kSkewed = 4 * kSkewFloats * sizeof(float),
-                     kOwn = 4 * kTileBytes<DP, grad_keys(DP)> + kHeldPassages * sizeof(int2) + 256;  // 256: of __syncthreads_or
-    if (a.bias.table && (blocks <= kUnits || 2 * (kOwn + kSkewed + lds) <= kLds)) {
-        kernel = grad_q_kernel<E, DP, kSkewedSums>;
-        lds += kSkewed;
-    }
+    const size_t lds = a.bias.table ? 5 * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
+    auto kernel = a.bias.table ? grad_q_kernel<E, DP, true> : grad_q_kernel<E, DP, false>;
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
     return hipGetLastError();
 }

@@ -15,9 +15,7 @@
 // quarter of the rate: the matrix cores are busy for 28 % of the time and the other instructions set the pace (more waves a
 // SIMD, which leaves each fewer registers, 77 us). 4096 tokens over 16 x 512, 16 heads of 128 over 4 key heads: 265 us,
 // 970 TFLOP/s; 4.7 others for a matrix instruction, matrix cores 45 %, LDS 34 %. 256 x 128 tokens with a bias, 12 heads of 64, the
-// keys of an encoder's own rows: 53 us for 164 MB, 3.1 TB/s: a block's two tiles are too few to hide its first loads.
-#include <type_traits>
-
+// keys of an encoder's own rows: 51 us for 164 MB, 3.2 TB/s: a block's two tiles are too few to hide its first loads.
 #include "attend_tile.hpp"
 
 namespace vk::attend {
@@ -110,13 +108,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub) s[sub] = E::mfma(straight<DP>(k, 32 * sub, 0, lane), qf[0], f32x16{});
             }
-            between_runs();
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-                for (int i = 1; i < kSteps; ++i) s[sub] = E::mfma(straight<DP>(k, 32 * sub, i, lane), qf[i], s[sub]);
-            feed<2 * kSteps - 2, 1, 4>();
-            between_runs();
+            products<2 * kSteps - 2, 1, 3>(
+                [&](int i) { return straight<DP>(k, 32 * (i / (kSteps - 1)), 1 + i % (kSteps - 1), lane); },
+                [&](int i, s16x8 x) { s[i / (kSteps - 1)] = E::mfma(x, qf[1 + i % (kSteps - 1)], s[i / (kSteps - 1)]); });
             __builtin_amdgcn_s_setprio(0);
             if constexpr (kLarge) {
 #pragma unroll
@@ -154,15 +148,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
                 total += s[r / 16][r % 16];
             }
             __builtin_amdgcn_s_setprio(1);
-            between_runs();
-#pragma unroll
-            for (int half = 0; half < 4; ++half) {
-                const s16x8 p = rounded<E>(s[half / 2], half % 2);
-#pragma unroll
-                for (int i = 0; i < kParts; ++i) o[i] = E::mfma(transposed<DP>(v, 16 * half, i, lane), p, o[i]);
-            }
-            feed<4 * kParts, 2, 4>();
-            between_runs();
+            s16x8 p;
+            products<4 * kParts, 2, 3>([&](int i) { return transposed<DP>(v, 16 * (i / kParts), i % kParts, lane); },
+                                       [&](int i, s16x8 x) {
+                                           if (i % kParts == 0) p = rounded<E>(s[i / kParts / 2], i / kParts % 2);
+                                           o[i % kParts] = E::mfma(x, p, o[i % kParts]);
+                                       });
             __builtin_amdgcn_s_setprio(0);
             if (more) {
                 ks.store(tile[now ^ 1][0]);
@@ -181,16 +172,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
         const float factor = total == 0.f ? 0.f : 1.f / total;
         char* out = static_cast<char*>(a.out.p) + (b * a.out.outer + token * a.out.middle + head * a.out.head) * 2;
 #pragma unroll
-        for (int i = 0; i < kParts; ++i)
-#pragma unroll
-            for (int quad = 0; quad < 4; ++quad) {
-                const int at = 32 * i + mfma_row(4 * quad, hi);
-                if (at >= a.d) continue;
-                typename E::T y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = (typename E::T)(o[i][4 * quad + j] * factor);
-                *reinterpret_cast<u32x2*>(out + at * 2) = *reinterpret_cast<u32x2*>(y);
-            }
+        for (int i = 0; i < kParts; ++i) store_column<E>(out, o[i], i, hi, a.d, factor);
         if (a.lse && hi == 0)
             a.lse[(static_cast<int64_t>(b) * a.heads + head) * a.tokens + token] = logarithm(top, total);
     } else {

@@ -2,6 +2,9 @@
 // keys, and the bias by distance.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "attend.hpp"
 
 namespace vk::attend {
@@ -58,21 +61,24 @@ __device__ __forceinline__ float both_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i);
+// A lane's and all lower lanes' sum.
+template <class T>
+__device__ __forceinline__ T wave_sums(T x) {
+    auto moved = [&](auto way, auto rows) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(way)::value, decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    const integral_constant<int, 0xf> all;
+    x += moved(integral_constant<int, 0x111>(), all);  // one, two, four, eight lanes up within 16
+    x += moved(integral_constant<int, 0x112>(), all);
+    x += moved(integral_constant<int, 0x114>(), all);
+    x += moved(integral_constant<int, 0x118>(), all);
+    x += moved(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // lane 15 of the first and third 16 to the next
+    x += moved(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // lane 31 to the upper half
     return x;
 }
-
-// A lane's and all lower lanes' sum.
-__device__ __forceinline__ int wave_sums(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // one, two, four, eight lanes up within 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 of the first and third 16 to the next
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
-    return x;
+__device__ __forceinline__ float wave_sum(float x) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wave_sums(x)), 63));
 }
 
 // Tiles in LDS: rows of DP 16-bit elements, 16 bytes apart. A ds_read_b128 of 16 consecutive lanes takes 16 bytes of 16 rows,
@@ -177,6 +183,23 @@ __device__ __forceinline__ s16x8 column(const AttendView& v, int64_t offset, boo
     const s16x8 x = *reinterpret_cast<const s16x8*>(static_cast<const char*>(v.p) + (there ? (offset + at) * 2 : 0));
     const s16x8 zero = {};
     return there ? x : zero;
+}
+
+// Writes a lane's column of a result, factor * x rounded, to elements 32 * part ... of its row. The halves of the wave that share a
+// column exchange every other four elements, so that a store is of 16 bytes (8 bytes each: 32 requests of 512 tokens, 12 heads of
+// 64, the keys' gradient 84 us where this takes 77).
+template <class E>
+__device__ __forceinline__ void store_column(char* row, const f32x16& x, int part, int hi, int d, float factor) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        typename E::T y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = (typename E::T)(x[8 * p + j] * factor);
+        const u32x4 z = *reinterpret_cast<u32x4*>(y);
+        const auto a = __builtin_amdgcn_permlane32_swap(z[0], z[2], false, false), b = __builtin_amdgcn_permlane32_swap(z[1], z[3], false, false);
+        const int at = 32 * part + 16 * p + 8 * hi;
+        if (at < d) *reinterpret_cast<u32x4*>(row + at * 2) = u32x4{a[0], b[0], a[1], b[1]};
+    }
 }
 
 // What lanes of a wave wrote to LDS before is there for its other lanes after.
@@ -402,21 +425,31 @@ __device__ __forceinline__ void each_bias(const float* held, int far, int x0, in
     }
 }
 
-// Instruction order of a run of `n` products of the matrix cores whose first operands come from LDS, `reads` reads each: the
-// reads are kept `most` products in front, as a read takes about as long as three to four products, and `others` vector
-// instructions of another part of the tile, that runs beside it, follow each product.
-template <int n, int reads, int most, int others = 0>
-__device__ __forceinline__ void feed() {
-    constexpr int ahead = most < n ? most : n;
-    __builtin_amdgcn_sched_group_barrier(0x100, reads * ahead, 0);
-#pragma unroll
-    for (int i = 0; i < n; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (i < n - ahead) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
-        if (others) __builtin_amdgcn_sched_group_barrier(0x002, others, 0);
-    }
-}
-// Where one run ends and the next begins.
+// Where one run of instructions ends and the next begins.
 __device__ __forceinline__ void between_runs() { __builtin_amdgcn_sched_barrier(0); }
+// A run of N products of the matrix cores whose first operands come from LDS, READS reads each: read(i) is kept MOST products
+// in front of product(i, ...), as a read takes about as long as three to four products. The order is asked of the compiler, and
+// written out besides: where a kernel is short of registers the compiler goes back to the order as written, and with each read
+// right before its product the queries' gradient of the wide tables took a tenth longer.
+template <int N, int READS, int MOST, class R, class P>
+__device__ __forceinline__ void products(R&& read, P&& product) {
+    constexpr int ahead = MOST < N ? MOST : N;
+    between_runs();
+    s16x8 first[ahead];
+#pragma unroll
+    for (int i = 0; i < ahead; ++i) first[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        product(i, first[i % ahead]);
+        if (i + ahead < N) first[i % ahead] = read(i + ahead);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * ahead, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + ahead < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    between_runs();
+}
 
 }  // namespace vk::attend
