@@ -84,6 +84,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
     const bool used = c < columns;
     const int64_t row = (static_cast<int64_t>(b) * a.heads + head) * a.tokens + token;
     auto at = [&](const AttendView& v) { return b * v.outer + token * v.middle + head * v.head; };
+    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
+    const int2 entry = places.look(a, b, thread);  // first of all, as the keys' loads wait for it
     s16x8 qf[kSteps], df[kSteps], of[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, at(a.q), used, i, hi, a.d);
@@ -91,9 +93,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
     for (int i = 0; i < kSteps; ++i) df[i] = column(g.d_out, at(g.d_out), used, i, hi, a.d);
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) of[i] = column(a.out, at(a.out), used, i, hi, a.d);
-    float2 lse = used ? a.lse[row] : make_float2(-INFINITY, 0.f);
-    const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
-    places.fill(a, b, found, thread, 256);
+    float2 lse = a.lse[used ? row : 0];
+    places.put(entry, found, thread);
 
     f32x16 dq[kParts];
 #pragma unroll
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
     KeyWalk<kSlots> walk(a, places, found, kv_head);
     bool more = walk.next();
     int now = 0;
-    if (more) walk.load(ks, vs);  // before the biases: what they wait for is under way with it
+    if (more) walk.load(ks, vs);
     int position = 0;
     float below = 0.f, above = 0.f;
     bool large = false;
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
     delta = both_sum(delta);
     if (used && hi == 0 && split == 0) g.delta[row] = delta;
     // rows without a key, and columns past the last: exp(x - inf) = 0
-    lse = make_float2(lse.x == -INFINITY ? INFINITY : lse.x, lse.y * -kLog2e);
+    lse = make_float2(!used || lse.x == -INFINITY ? INFINITY : lse.x, used ? lse.y * -kLog2e : 0.f);
     const float scale_log2 = a.scale * kLog2e;
     if (more) {
         ks.store(tile[0][0]);

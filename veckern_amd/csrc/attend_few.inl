@@ -42,10 +42,11 @@ __global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(A
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
     const int64_t q = b * a.q.outer + token * a.q.middle + head * a.q.head;
+    const int2 entry = places.look(a, b, thread);  // first of all, as the keys' loads wait for it
     s16x8 qf[kSteps];
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
-    places.fill(a, b, found, thread, kThreads);
+    places.put(entry, found, thread);
     const float* held = nullptr;
     int position = 0;
     if constexpr (BIAS) {

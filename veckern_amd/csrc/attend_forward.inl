@@ -41,11 +41,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
     const int token = c / a.pack, head = group * a.pack + c % a.pack;
     const bool used = c < columns;
     const int64_t q = b * a.q.outer + token * a.q.middle + head * a.q.head;
-    s16x8 qf[kSteps];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
     const Places places(a, split * a.tiles_per_split * kSlots, a.tiles_per_split * kSlots);
-    places.fill(a, b, found, thread, 256);
+    // first what the keys' loads wait for; then all other loads are under way together
+    places.put(places.look(a, b, thread), found, thread);
 
     f32x16 o[kParts];
 #pragma unroll
@@ -59,7 +57,10 @@ __global__ __launch_bounds__(256, DP <= 64 ? 3 : 2) void forward_kernel(AttendAr
     KeyWalk<kSlots> walk(a, places, found, kv_head);
     bool more = walk.next();
     int now = 0;
-    if (more) walk.load(ks, vs);  // before the biases: what they wait for is under way with it
+    if (more) walk.load(ks, vs);
+    s16x8 qf[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) qf[i] = column(a.q, q, used, i, hi, a.d);
     const float* held = nullptr;
     int position = 0;
     bool large = false;

@@ -223,13 +223,15 @@ __device__ __forceinline__ float2 logarithm(float top, float total) {
 // One scalar-register value from a load whose address is the same in all lanes.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// The bank row of passage r of request b and how many positions it holds: none for a row outside the bank.
+// The bank row of passage r of request b and how many positions it holds: none for a row outside the bank. No branch follows the
+// loads, so that nothing waits for them here.
 __device__ __forceinline__ int2 find_row(const AttendArgs& a, int b, int r) {
     int row = b * a.passages + r, count = a.length;
     if (a.rows) row = a.rows[b * a.rows_outer + r * a.rows_step];
-    if (a.rows && (row < 0 || row >= a.bank)) return make_int2(0, 0);
-    if (a.lengths) count = min(max(a.lengths[row], 0), a.length);
-    return make_int2(row, count);
+    const bool there = row >= 0 && row < a.bank;
+    row = there ? row : 0;
+    if (a.lengths && a.bank) count = min(max(a.lengths[row], 0), a.length);
+    return make_int2(row, there ? count : 0);
 }
 // A request's keys are counted in places: slots of its passages, empty ones included, passage by passage. A block holds the rows
 // of the passages that its places [begin, end) lie in.
@@ -241,9 +243,12 @@ struct Places {
         end = min(from + count, per_row * a.passages);
         r0 = begin < end ? begin / per_row : 0;
     }
-    __device__ void fill(const AttendArgs& a, int b, int2* found, int thread, int threads) const {
-        if (begin < end)
-            for (int r = r0 + thread; r <= (end - 1) / per_row; r += threads) found[r - r0] = find_row(a, b, r);
+    // A thread's entry of the block's table; a block has a thread for each.
+    __device__ int2 look(const AttendArgs& a, int b, int thread) const {
+        return begin < end ? find_row(a, b, min(r0 + thread, (end - 1) / per_row)) : make_int2(0, 0);
+    }
+    __device__ void put(int2 entry, int2* found, int thread) const {
+        if (thread < kHeldPassages) found[thread] = entry;
     }
 };
 
