@@ -285,6 +285,26 @@ def test_gradients_against_differences():
         assert abs(slope - ours) <= allowed, (name, slope, ours, allowed)
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_gradients_of_rows_with_one_key(d):
+    """A softmax over one key is constant: no gradient reaches queries, keys or table, whatever the output was rounded to."""
+    from veckern_amd import attention
+
+    q, k, v, _, _, d_out = make(51, BF16, 3, 40, 1, 30, 4, 2, d)
+    lengths = torch.ones(3, dtype=torch.int32, device="cuda")
+    table = torch.randn(8, 4, generator=torch.Generator().manual_seed(52)).to(BF16).cuda()
+    bias = attention.RelativeBias(table, 10, True)
+    out, lse = attention.attend(q, k, v, lengths=lengths, bias=bias, return_lse=True)
+    grad = attention.attend_backward(d_out, q, k, v, out, lse, lengths=lengths, bias=bias)
+    # dP and the sum of P dP differ by what 32 bits leave: P is 1 up to 2^-18 (an exponent of at most 2^4, in steps of 2^-20,
+    # and the exponential's own error), so that |dS| <= 2^-17 |dP|
+    dp = (d_out.double().abs() * v[:, :1].double().abs().repeat_interleave(2, dim=2)).sum(-1)
+    most = float(dp.max()) * 2.0 ** -17
+    assert float(grad.queries.abs().max()) <= most * float(k.abs().max()) / d ** 0.5
+    assert float(grad.keys.abs().max()) <= most * 40 * 2 * float(q.abs().max()) / d ** 0.5
+    assert float(grad.table.abs().max()) <= most * 3 * 40
+
+
 def test_automatic_differentiation():
     from veckern_amd import attention
 

@@ -6,8 +6,9 @@
 // memory, no second copy of dQ in 32 bits, and the same bits from every run. P and dS are rounded to the inputs' type where
 // they become operands (the matrix instructions take 16 bits; in binary16 small dS need the loss scaling that training in
 // that type uses anyway); statistics, dP, delta and all sums are held in 32 bits. delta is taken from the rounded output, as that
-// is what a program has kept: its error, of 2^-9 of the output's size in bfloat16, is the same for all keys of a row, and shows
-// most in the table's gradient, whose terms of a row cancel. Taking it from P dP instead would cost two more products.
+// is what a program has kept: its error, of 2^-9 of the output's size in bfloat16, is the same for all keys of a row. It shows where
+// a row has few keys and dP - delta all but cancels; there, where one tile holds them all, delta is the sum of P dP, which is there
+// by then. With more tiles that would take two more products.
 //
 // Measured: 32 requests of 512 tokens over their own, 12 heads of 64, a two-sided bias: queries 93 us, keys 77 us (415 and 670
 // TFLOP/s of the products done), of which 30 and 14 us go by where no key is there: the reading of a block's own columns and
@@ -128,7 +129,6 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
         for (int j = 0; j < 8; ++j) delta = __builtin_fmaf(static_cast<float>(x[j]), static_cast<float>(y[j]), delta);
     }
     delta = both_sum(delta);
-    if (used && hi == 0 && split == 0) g.delta[row] = delta;
     // rows without a key, and columns past the last: exp(x - inf) = 0
     lse = make_float2(!used || lse.x == -INFINITY ? INFINITY : lse.x, used ? lse.y * -kLog2e : 0.f);
     const float scale_log2 = a.scale * kLog2e;
@@ -157,14 +157,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
                                        dq[i % kParts] = E::mfma(x, y, dq[i % kParts]);
                                    });
     };
-    auto run = [&](auto kind) {
-        constexpr bool kLarge = decltype(kind)::value;
+    // kAlone: one tile holds all keys of the rows
+    auto run = [&](auto kind, auto single) {
+        constexpr bool kLarge = decltype(kind)::value, kAlone = decltype(single)::value;
         while (more) {
             Slot slots[kSlots];
 #pragma unroll
             for (int i = 0; i < kSlots; ++i) slots[i] = walk.slots[i];
             const bool full = walk.run || whole(slots);
-            more = walk.next();
+            more = !kAlone && walk.next();
             if (more) walk.load(ks, vs);
             const int2 at_keys = reach(slots);
             k = tile[now][0];
@@ -201,6 +202,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
                 const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
 #pragma unroll
                 for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_fmaf(s[r / 16][r % 16], scale_log2, shift);
+            }
+            if constexpr (kAlone) {
+                float sum = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16 * kSubs; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(s[r / 16][r % 16]);
+                    sum = __builtin_fmaf(slot_row(r, hi) < slots[r / 8].left ? p : 0.f, dp[r / 16][r % 16], sum);
+                }
+                delta = both_sum(sum);
             }
 #pragma unroll
             for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
@@ -246,9 +256,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
             now ^= 1;
         }
     };
-    if (BIAS && large) run(std::integral_constant<bool, BIAS>());
-    else run(std::false_type());
+    auto each = [&](auto single) {
+        if (BIAS && large) run(std::integral_constant<bool, BIAS>(), single);
+        else run(std::false_type(), single);
+    };
+    KeyWalk<kSlots> ahead = walk;
+    if (a.splits == 1 && !ahead.next()) each(std::true_type());
+    else each(std::false_type());
 
+    if (used && hi == 0 && split == 0) g.delta[row] = delta;
     if (used && a.splits > 1) {
         float* part = a.part + (((static_cast<int64_t>(split) * a.batch + b) * groups + group) * columns + c) * a.d;
 #pragma unroll
