@@ -20,6 +20,7 @@ constexpr int grad_keys(int d) { return d <= 64 ? 64 : 32; }  // keys of a tile 
 constexpr int grad_queries(int d) { return d <= 64 ? 64 : 32; }  // queries of a tile of the keys' and values' gradient
 constexpr int kColumns = 128;        // query columns of a block of the tile kernels
 constexpr int kUnits = 256;          // compute units of the card
+constexpr int kMostBlocks = (1 << 30) - 1;  // of a grid that xcd_place() orders, which doubles the size of a group of blocks
 
 // A tensor [outer][middle][head][d]: element strides, d contiguous.
 struct AttendView {

@@ -773,7 +773,7 @@ template <class E, int DP>
 hipError_t launch_grad_q(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns * (a.heads / a.pack) * a.batch * a.splits;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks > kMostBlocks) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? 5 * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     auto kernel = a.bias.table ? grad_q_kernel<E, DP, true> : grad_q_kernel<E, DP, false>;
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(g);
@@ -785,7 +785,7 @@ hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t slots = static_cast<int64_t>((a.length + kSlot - 1) / kSlot) * a.passages;
     const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch * g.kv_splits;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks > kMostBlocks) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     if constexpr (DP <= 64) {  // two waves for 32 keys: 170 us where one took 142 then (4 x 2048 tokens, 12 heads of 64)
         auto kernel = a.bias.table ? grad_kv_kernel<E, DP, true> : grad_kv_kernel<E, DP, false>;

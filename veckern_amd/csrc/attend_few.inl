@@ -199,7 +199,7 @@ __global__ __launch_bounds__(64 * kFewWaves, DP <= 64 ? 4 : 2) void few_kernel(A
 template <class E, int DP>
 hipError_t launch_few(const AttendArgs& a, hipStream_t stream) {
     const int64_t blocks = (static_cast<int64_t>(a.tokens) * a.pack + 31) / 32 * a.splits * (a.heads / a.pack) * a.batch;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks > kMostBlocks) return hipErrorInvalidValue;
     const size_t lds = kFewTiles<DP> + kHeldPassages * sizeof(int2) +
                        (a.bias.table ? a.pack * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0);
     auto kernel = a.bias.table ? few_kernel<E, DP, true> : few_kernel<E, DP, false>;

@@ -195,7 +195,7 @@ template <class E, int DP>
 hipError_t launch_forward(const AttendArgs& a, hipStream_t stream) {
     const int64_t column_tiles = (static_cast<int64_t>(a.tokens) * a.pack + kColumns - 1) / kColumns;
     const int64_t blocks = column_tiles * a.splits * (a.heads / a.pack) * a.batch;
-    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (blocks > kMostBlocks) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? a.pack * (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     auto kernel = a.bias.table ? forward_kernel<E, DP, true> : forward_kernel<E, DP, false>;
     kernel<<<static_cast<unsigned>(blocks), 256, lds, stream>>>(a);
