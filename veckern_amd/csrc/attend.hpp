@@ -67,6 +67,10 @@ struct AttendGradArgs {
     void* d_table = nullptr;      // [buckets][heads], contiguous
     // Runs of a key head's query tiles (head by head) that different blocks take for d_k and d_v.
     int kv_splits = 1, kv_tiles_per_split = 0;
+    // Blocks of 256 threads that join d_q's parts and the table's partial sums, of which there are table_parts: those of d_q first.
+    // They stand behind the blocks of the keys' gradient, which waits for what they need anyway, or, for rows of a bank, in a launch
+    // of their own (3 requests of 77 tokens over 5 x 131, 6 heads of 80, bias, forward and backward: 51 us with that launch, 47 so).
+    int join_q = 0, join_table = 0, table_parts = 0;
     float* kv_part = nullptr;     // kv_splits > 1: workspace [d_k, d_v][kv_splits][bank][length][kv_heads][d]
 };
 
@@ -78,7 +82,7 @@ hipError_t launch_attend_combine(const AttendArgs& a, int type, hipStream_t stre
 // Writes d_q, or its parts, delta and the table's partial sums.
 hipError_t launch_attend_grad_q(const AttendGradArgs& g, int type, hipStream_t stream);
 hipError_t launch_attend_grad_kv(const AttendGradArgs& g, int type, hipStream_t stream);
-// Joins what the splits wrote, and the table's partial sums.
-hipError_t launch_attend_grad_join(const AttendGradArgs& g, int type, int parts, hipStream_t stream);
+// Joins d_q's parts and the table's sums if `queries`, and the parts of d_k and d_v if there are any.
+hipError_t launch_attend_grad_join(const AttendGradArgs& g, int type, bool queries, hipStream_t stream);
 
 }  // namespace vk

@@ -392,7 +392,12 @@ __global__ __launch_bounds__(256, 2) void grad_kv_kernel(AttendGradArgs g) {
     const int thread = threadIdx.x, lane = thread % 64, wave = thread / 64, hi = lane / 32;
     const int share = a.heads / a.kv_heads, per_row = (a.length + kSlot - 1) / kSlot;
     const int key_tiles = (per_row * a.passages + kColumns / kSlot - 1) / (kColumns / kSlot);
-    int place = xcd_place(blockIdx.x, gridDim.x, key_tiles * g.kv_splits);
+    const int keys = key_tiles * g.kv_splits * a.kv_heads * a.batch;
+    if (static_cast<int>(blockIdx.x) >= keys) {
+        join_queries<E>(g, blockIdx.x - keys, thread);
+        return;
+    }
+    int place = xcd_place(blockIdx.x, keys, key_tiles * g.kv_splits);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
     int split = 0;
@@ -600,7 +605,13 @@ __global__ __launch_bounds__(512, 2) void grad_kv_pair_kernel(AttendGradArgs g) 
     const bool second = uniform(thread / 256) != 0;
     const int share = a.heads / a.kv_heads, per_row = (a.length + kSlot - 1) / kSlot;
     const int key_tiles = (per_row * a.passages + kColumns / kSlot - 1) / (kColumns / kSlot);
-    int place = xcd_place(blockIdx.x, gridDim.x, key_tiles * g.kv_splits);
+    const int keys = key_tiles * g.kv_splits * a.kv_heads * a.batch;
+    if (static_cast<int>(blockIdx.x) >= keys) {
+        const int block = 2 * (blockIdx.x - keys) + (second ? 1 : 0);
+        if (block < g.join_q + g.join_table) join_queries<E>(g, block, thread % 256);
+        return;
+    }
+    int place = xcd_place(blockIdx.x, keys, key_tiles * g.kv_splits);
     const int key_tile = place % key_tiles;
     place /= key_tiles;
     int split = 0;
@@ -784,7 +795,9 @@ template <class E, int DP>
 hipError_t launch_grad_kv(const AttendGradArgs& g, hipStream_t stream) {
     const AttendArgs& a = g.a;
     const int64_t slots = static_cast<int64_t>((a.length + kSlot - 1) / kSlot) * a.passages;
-    const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch * g.kv_splits;
+    const int64_t joined = static_cast<int64_t>(g.join_q) + g.join_table;
+    const int64_t blocks = (slots + kColumns / kSlot - 1) / (kColumns / kSlot) * a.kv_heads * a.batch * g.kv_splits +
+                           (DP <= 64 ? joined : (joined + 1) / 2);
     if (blocks > kMostBlocks) return hipErrorInvalidValue;
     const size_t lds = a.bias.table ? (2 * a.bias.far + 2 * kPad + 1) * sizeof(float) : 0;
     if constexpr (DP <= 64) {  // two waves for 32 keys: 170 us where one took 142 then (4 x 2048 tokens, 12 heads of 64)

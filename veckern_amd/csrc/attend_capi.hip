@@ -343,8 +343,14 @@ VK_EXPORT int vk_attend_backward(const vk_attention* x, const vk_attention_grad*
         a.part = reinterpret_cast<float*>(at + delta_bytes(a) + table_bytes(a));
         g.kv_part = reinterpret_cast<float*>(at + delta_bytes(a) + table_bytes(a) + part_bytes(a));
         const auto on = static_cast<hipStream_t>(stream);
+        const int64_t join_q = a.splits > 1 ? static_cast<int64_t>((query_rows(a) * (a.d / 4) + 255) / 256) : 0;
+        valid(join_q < vk::kMostBlocks, "a size is too large");
+        g.join_q = static_cast<int>(join_q);
+        g.join_table = a.bias.table ? (a.heads * a.bias.buckets + 3) / 4 : 0;
+        g.table_parts = table_parts(a);
+        const bool states = !x->rows && x->bank && x->length;
         if (query_rows(a)) VK_HIP(vk::launch_attend_grad_q(g, x->type, on));
-        if (!x->rows && x->bank && x->length) VK_HIP(vk::launch_attend_grad_kv(g, x->type, on));
-        if (a.bias.table || (a.splits > 1 && query_rows(a)) || g.kv_splits > 1) VK_HIP(vk::launch_attend_grad_join(g, x->type, table_parts(a), on));
+        if (states) VK_HIP(vk::launch_attend_grad_kv(g, x->type, on));
+        VK_HIP(vk::launch_attend_grad_join(g, x->type, !states, on));
     });
 }

@@ -457,4 +457,37 @@ __device__ __forceinline__ void products(R&& read, P&& product) {
     between_runs();
 }
 
+// A block of 256 threads of those that follow the queries' gradient: d_q = scale * sum of the splits' parts, four elements a thread,
+// or the table's gradient, one wave per (bucket, head).
+template <class E>
+__device__ __forceinline__ void join_queries(const AttendGradArgs& g, int block, int thread) {
+    const AttendArgs& a = g.a;
+    if (block < g.join_q) {
+        const int groups = a.heads / a.pack, columns = a.tokens * a.pack, quads = a.d / 4;
+        const int64_t rows = static_cast<int64_t>(a.batch) * groups * columns, at = static_cast<int64_t>(block) * 256 + thread;
+        if (at >= rows * quads) return;
+        const int64_t row = at / quads;
+        const int e = static_cast<int>(at - row * quads) * 4;
+        f32x4 x{};
+#pragma unroll 4
+        for (int i = 0; i < a.splits; ++i) x += *reinterpret_cast<const f32x4*>(a.part + (i * rows + row) * a.d + e);
+        const int c = row % columns, group = row / columns % groups, b = row / columns / groups;
+        const int token = c / a.pack, head = group * a.pack + c % a.pack;
+        typename E::T z[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[j] = (typename E::T)(x[j] * g.scale);
+        char* out = static_cast<char*>(g.d_q.p) + (b * g.d_q.outer + token * g.d_q.middle + head * g.d_q.head + e) * 2;
+        *reinterpret_cast<u32x2*>(out) = *reinterpret_cast<u32x2*>(z);
+        return;
+    }
+    const int lane = thread % 64, at = (block - g.join_q) * 4 + thread / 64;
+    if (at >= a.heads * a.bias.buckets) return;
+    const int head = at % a.heads, bucket = at / a.heads;
+    float x = 0.f;
+#pragma unroll 4
+    for (int i = lane; i < g.table_parts; i += 64) x += g.table_part[(static_cast<int64_t>(i) * a.heads + head) * a.bias.buckets + bucket];
+    x = wave_sum(x);
+    if (lane == 0) static_cast<typename E::T*>(g.d_table)[at] = (typename E::T)x;
+}
+
 }  // namespace vk::attend
