@@ -13,9 +13,9 @@
 // Measured: 32 requests of 512 tokens over their own, 12 heads of 64, a two-sided bias: queries 93 us, keys 77 us (415 and 670
 // TFLOP/s of the products done), of which 30 and 14 us go by where no key is there: the reading of a block's own columns and
 // the writing of its results, which all blocks do at about the same time; 4 of 2048 tokens: 135 and 131 us. 2 of 2048 tokens over
-// 4 x 2048, 16 heads of 128, no bias: 395 and 610 us (1040 and 900 TFLOP/s). With heads of 64 the matrix cores are busy for 25 % and 35 % of the time, and the rest is VALU:
-// exponentials, bias and the table's sums; with 128 for 50 % and 39 %, LDS for 33 % and 37 %, and what is left are waits: of a tile
-// for its barrier, with two waves a SIMD, which registers limit.
+// 4 x 2048, 16 heads of 128, no bias: 395 and 610 us (1040 and 900 TFLOP/s). With heads of 64 the matrix cores are busy for 24 %
+// and 35 % of the time, and the rest is VALU: exponentials, bias and the table's sums; with 128 for 51 % and 40 %, LDS for 34 % and
+// 38 %, and what is left are waits: of a tile for its barrier, with two waves a SIMD, which registers limit.
 #include "attend_tile.hpp"
 
 namespace vk::attend {
@@ -195,9 +195,10 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
             if constexpr (kLarge) {
 #pragma unroll
                 for (int sub = 0; sub < kSubs; ++sub)
-                    each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position, [&](int r, float x) {
-                        s[sub][r] = __builtin_fmaf(__builtin_fmaf(s[sub][r], a.scale, x) - lse.x, kLog2e, lse.y);
-                    });
+                    each_bias<1>(held, a.bias.far, slots[2 * sub].first + hi - position, slots[2 * sub + 1].first + hi - position,
+                                 [&](int r, float x) {
+                                     s[sub][r] = __builtin_fmaf(__builtin_fmaf(s[sub][r], a.scale, x) - lse.x, kLog2e, lse.y);
+                                 });
             } else {
                 const float shift = __builtin_fmaf(apart - lse.x, kLog2e, lse.y);
 #pragma unroll
@@ -213,7 +214,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
                 delta = both_sum(sum);
             }
 #pragma unroll
-            for (int r = 0; r < 16 * kSubs; ++r) s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
+            for (int r = 0; r < 16 * kSubs; ++r)
+                s[r / 16][r % 16] = __builtin_amdgcn_exp2f(s[r / 16][r % 16]) * (dp[r / 16][r % 16] - delta);
             if (!full) {
 #pragma unroll
                 for (int r = 0; r < 16 * kSubs; ++r)
@@ -309,7 +311,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 3 : 2) void grad_q_kernel(AttendGra
 #pragma unroll
             for (int i = 1; i < 8; i *= 2) x += __shfl_xor(x, i);
             if (thread % 8 == 0 && bucket < s.buckets)
-                g.table_part[(((static_cast<int64_t>(split) * a.batch + b) * column_tiles + column_tile) * a.heads + head) * s.buckets + bucket] = x;
+                g.table_part[(((static_cast<int64_t>(split) * a.batch + b) * column_tiles + column_tile) * a.heads + head) * s.buckets +
+                             bucket] = x;
         }
     }
 }
@@ -338,7 +341,8 @@ __device__ __forceinline__ KeySlot key_slot(const AttendArgs& a, int b, int slot
         for (int i = 0; i < 2; ++i) {
             const uint64_t at = __ballot(before + upto > slot + i);
             if (found > i || !at) continue;
-            const int l = __builtin_ctzll(at), n = slot + i - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(slots, l));
+            const int l = __builtin_ctzll(at);
+            const int n = slot + i - before - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(slots, l));
             x[i] = {b * a.passages + r0 + l, n * kSlot, __builtin_amdgcn_readlane(count, l) - n * kSlot};
             found = i + 1;
         }

@@ -65,7 +65,8 @@ __device__ __forceinline__ float both_sum(float x) {
 template <class T>
 __device__ __forceinline__ T wave_sums(T x) {
     auto moved = [&](auto way, auto rows) {
-        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(way)::value, decltype(rows)::value, 0xf, false));
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(way)::value,
+                                                                 decltype(rows)::value, 0xf, false));
     };
     using std::integral_constant;
     const integral_constant<int, 0xf> all;
@@ -196,7 +197,8 @@ __device__ __forceinline__ void store_column(char* row, const f32x16& x, int par
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = (typename E::T)(x[8 * p + j] * factor);
         const u32x4 z = *reinterpret_cast<u32x4*>(y);
-        const auto a = __builtin_amdgcn_permlane32_swap(z[0], z[2], false, false), b = __builtin_amdgcn_permlane32_swap(z[1], z[3], false, false);
+        const auto a = __builtin_amdgcn_permlane32_swap(z[0], z[2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(z[1], z[3], false, false);
         const int at = 32 * part + 16 * p + 8 * hi;
         if (at < d) *reinterpret_cast<u32x4*>(row + at * 2) = u32x4{a[0], b[0], a[1], b[1]};
     }
