@@ -4,9 +4,9 @@
 // many loads in flight: a wave has its next tile's K and V (16 KB at 128 elements a head) under way while it works on one. Nothing
 // waits at a barrier in between. Products, roundings and the raised maximum are those of the tile kernel (attend_forward.inl).
 //
-// Measured, bound by the reading: one token of each of 32 requests over 100 x 256 positions, 8 key heads of 128: 550 us for
-// 2.2 GB of different states, 4.0 TB/s (a large copy: 5.0); 64 requests over 10 x 100, 12 heads of 128: 80 us for 393 MB, 4.9 TB/s; of
-// 64: 37 us, 5.3 TB/s with what the caches hold from call to call. 64 over 10 ragged rows of up to 100, 4 key heads of 128: 19 us
+// Measured, bound by the reading: one token of each of 32 requests over 100 x 256 positions, 8 key heads of 128: 530 us for
+// 3.4 GB, 2.2 of them different, 6.3 TB/s; 128 requests over 10 x 200, 12 heads of 128: 260 us for 1.6 GB, 6.0 TB/s; 256 over as many,
+// heads of 64: 290 us for 1.6 GB, 5.4 TB/s (a large copy: 5.0). 64 over 10 ragged rows of up to 100, 4 key heads of 128: 19 us
 // for 68 MB, one round of one block a compute unit. One request over 10 x 64: 8 us, latency: records, lengths, states and the
 // join follow each other.
 #include <atomic>
